@@ -50,6 +50,26 @@ cudaError_t embedding_fwd(const int64_t* idx, const float* W, float* x, int64_t 
 cudaError_t embedding_bwd(const int64_t* idx, const float* dx, float* dW, int64_t N, int d, int64_t V, int64_t v0,
                           cudaStream_t st);
 
+// ---------------------------------------------------------------- rotary positions (rope/rotary.cu)
+// Heads (B, T, heads, hd) by element strides, unit stride along hd; out may be in.
+struct RopeHeads {
+  const void* in;
+  void* out;
+  int heads;
+  int64_t isb, ist, ish, osb, ost, osh;
+};
+struct RopeArgs {
+  RopeHeads q, k;  // k.heads == 0: no k
+  int B, T, hd, rd;
+  const void* pos;  // int32 or int64 (pos64) positions by strides, or nullptr: 0 .. T - 1
+  bool pos64;
+  int64_t psb, pst;
+  const float* table;  // (kRopeTableRows, rd / 2, 2) cosines and sines: see rotary.cu
+  bool interleaved, inverse;
+};
+constexpr int kRopeTableRows = 4096;
+cudaError_t rotary(const RopeArgs& a, int kind, cudaStream_t st);  // kind: 0 bf16, 1 fp16, 2 fp32
+
 // ---------------------------------------------------------------- optimizer
 struct AdamHyper {
   float b1, b2, eps, wd, grad_scale;
@@ -58,6 +78,38 @@ cudaError_t adamw_step(float* p, float* g, float* m, float* v, void* p16, int64_
                        const int* step, AdamHyper h, bool zero_grad, cudaStream_t st, int max_blocks = 0);
 cudaError_t cast_bf16(const float* x, void* y, int64_t n, cudaStream_t st, int max_blocks = 0);
 
+// AdamW over many tensors (adamw/adamw_multi.cu). The states of all tensors lie in one buffer each,
+// in blocks of 256 values; a tensor starts at its first_block and fills whole blocks.
+struct MultiTensor {
+  float* p;
+  void* g;
+  void* p16;  // bf16 copy, or nullptr
+  int64_t n;
+  int32_t first_block;  // in the states
+  int32_t first_work;   // in the launch: blocks of the tensors before it (set by the launcher)
+  float wd;
+};
+struct MultiState {
+  void *m, *v;        // 8 bits: codes; 32 bits: fp32
+  uint8_t *ms, *vs;   // 8 bits: one exponent byte per block
+};
+struct MultiHyper {
+  float b1, c1, b2, c2, eps, grad_scale;  // c1 = 1 - b1, c2 = 1 - b2
+  const float* lr;
+  const float* grad_scale_dev;  // multiplies grad_scale, or nullptr
+  int* step;                    // steps taken before this one; counted by it
+  unsigned* ticket;             // zero between steps
+  uint32_t seed;
+  bool zero_grad;
+};
+cudaError_t adamw_multi(const MultiTensor* t, int count, bool grad_bf16, int bits, const MultiHyper& h, const MultiState& s,
+                        cudaStream_t st);
+// n: a multiple of 8, outputs bf16 or fp32 (f32).
+cudaError_t adamw_state_values(const uint8_t* m, const uint8_t* ms, const uint8_t* v, const uint8_t* vs, void* mo, void* vo,
+                               bool f32, int64_t n, cudaStream_t st);
+cudaError_t adamw_encode_states(const float* m, const float* v, uint8_t* mc, uint8_t* ms, uint8_t* vc, uint8_t* vs,
+                                int64_t blocks, cudaStream_t st);
+
 // ---------------------------------------------------------------- cross entropy rows
 cudaError_t ce_fwd_rows(const void* logits, int64_t ld, const int64_t* tgt, float* lse, float* loss, int64_t R, int V,
                         cudaStream_t st);
@@ -65,6 +117,57 @@ cudaError_t ce_bwd_rows(void* logits, int64_t ld, const int64_t* tgt, const floa
                         float scale, int64_t R, int V, cudaStream_t st);
 cudaError_t ce_combine(const float* part, const float* tlogit, const int64_t* tgt, float* lse, float* loss, int M,
                        int nblk, int V, cudaStream_t st);
+
+// ---------------------------------------------------------------- post-training losses (loss/loss_rows.cu)
+// A (B, T) array addressed by element strides (0 broadcasts); p == nullptr: not given.
+template <typename E>
+struct Strided {
+  const E* p;
+  int64_t sb, st;
+};
+// Logits z (B, T, V) of dtype 0 bf16 / 1 fp16 / 2 fp32, unit stride along V, with target ids and
+// the mask of the tokens that count.
+struct TokenBatch {
+  const void* z;
+  int dtype, B, T, V;
+  int64_t zsb, zst;
+  Strided<int64_t> tgt;
+  Strided<uint8_t> mask;
+};
+enum LossReduction : int { LOSS_TOKEN = 0, LOSS_SEQUENCE = 1, LOSS_SUM = 2 };
+enum PreferenceKind : int { PREF_SIGMOID = 0, PREF_HINGE = 1, PREF_IPO = 2 };
+struct PolicyArgs {
+  Strided<float> old, adv, ref;  // old: nullptr means the current log-probabilities
+  float clip_lo, clip_hi, kl_coef;
+  int reduction;
+};
+struct PreferenceArgs {
+  Strided<float> ref;
+  float beta, smoothing;
+  int kind;
+  bool average;
+};
+struct RowOut {
+  float* logp;       // (B T)
+  float2* stats;     // (B T) maximum and sum of exp(z - maximum), or nullptr
+  float* loss;       // (1)
+  float* loss_rows;  // scratch: (B T) policy, (B / 2) preference
+  float* coef;       // (B T) slope of the loss in each token's log-probability
+  float* rewards;    // (B) preference: beta times each sequence's gain
+  int* count;        // (B) scratch of the policy loss
+  unsigned* ticket;  // (1) scratch
+  void* dz;          // gradient rows, the logits' type, or nullptr; may be z itself
+  int64_t sb, st;    // their element strides
+  const float* grad_out;  // device scalar that multiplies the gradient, or nullptr
+};
+cudaError_t logprob_rows(const TokenBatch& a, const RowOut& o, cudaStream_t st);
+cudaError_t policy_rows(const TokenBatch& a, const PolicyArgs& q, const RowOut& o, cudaStream_t st);
+cudaError_t policy_tokens(const TokenBatch& a, const PolicyArgs& q, const float* logp, const RowOut& o, cudaStream_t st);
+// ticket_ready: the ticket is zero already (logprob_rows leaves it so), else it is cleared here.
+cudaError_t preference_tokens(const TokenBatch& a, const PreferenceArgs& q, const float* logp, const RowOut& o,
+                              bool ticket_ready, cudaStream_t st);
+// dz from coef and stats; skip_one: dz holds it already where *grad_out is 1.
+cudaError_t grad_rows(const TokenBatch& a, const RowOut& o, bool skip_one, cudaStream_t st);
 
 // ---------------------------------------------------------------- GEMM
 enum EpiKind : int {

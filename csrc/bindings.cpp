@@ -5,10 +5,27 @@
 // of api.h on the current CUDA stream. Launch errors become Python exceptions.
 #include <torch/extension.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
 
 #include "api.h"
 
-#define CHECK(cond, ...) TORCH_CHECK(cond, "llmt: ", __VA_ARGS__)
+// Messages are put together here, numbers by std::to_string: a number streamed into TORCH_CHECK's
+// message ends the process where torch and this module bring two copies of the C++ library's locales.
+template <typename... A>
+std::string message(const A&... a) {
+  std::string s = "llmt: ";
+  auto one = [&s](const auto& x) {
+    using X = std::decay_t<decltype(x)>;
+    if constexpr (std::is_same_v<X, at::ScalarType>) s += c10::toString(x);
+    else if constexpr (std::is_arithmetic_v<X>) s += std::to_string(x);
+    else s += x;
+  };
+  (one(a), ...);
+  return s;
+}
+#define CHECK(cond, ...) TORCH_CHECK(cond, message(__VA_ARGS__))
 #define CHECK_DT(t, dt) CHECK((t).scalar_type() == (dt), #t " has dtype ", (t).scalar_type(), ", expected ", (dt))
 
 namespace {
@@ -24,6 +41,8 @@ void ok(cudaError_t e, const char* what) {
 }
 
 void on_device(const at::Tensor& t, const char* name);
+int float_kind(const at::Tensor& t, const char* name);
+void all_on_device(std::initializer_list<std::pair<const c10::optional<at::Tensor>, const char*>> given);
 
 void cuda2d(const at::Tensor& t, const char* name) {
   on_device(t, name);
@@ -155,6 +174,89 @@ void embedding_bwd(at::Tensor idx, at::Tensor dx, at::Tensor dW, int64_t v0) {
      "embedding_bwd");
 }
 
+// ---------------------------------------------------------------- rotary positions
+llmt::RopeHeads rope_heads(const at::Tensor& x, const at::Tensor& y) {
+  return {x.data_ptr(), y.data_ptr(), (int)x.size(2), x.stride(0), x.stride(1), x.stride(2), y.stride(0), y.stride(1), y.stride(2)};
+}
+
+// Rotates q and (when given) k, (B, T, heads, hd) with unit stride along hd, into q_out / k_out:
+// new contiguous tensors, or given ones, which may be q and k themselves.
+std::vector<at::Tensor> rotary(at::Tensor q, c10::optional<at::Tensor> k, c10::optional<at::Tensor> positions, at::Tensor table,
+                               int64_t rotary_dim, bool interleaved, bool inverse, c10::optional<at::Tensor> q_out,
+                               c10::optional<at::Tensor> k_out) {
+  const bool has_k = k.has_value() && k->defined();
+  CHECK(q.dim() == 4, "rotary: q must be (batch, tokens, heads, head_dim)");
+  const int64_t B = q.size(0), T = q.size(1), hd = q.size(3);
+  const int kind = float_kind(q, "q");
+  CHECK(rotary_dim > 0 && rotary_dim % 2 == 0 && rotary_dim <= hd, "rotary: rotary_dim must be even and at most head_dim");
+  CHECK(B <= 0x7fffffff && T <= 0x7fffffff && B * T <= 0x7fffffff, "rotary: more than 2^31 - 1 tokens");
+  CHECK(table.scalar_type() == at::kFloat && table.is_contiguous() && table.dim() == 3 &&
+            table.size(0) == llmt::kRopeTableRows && table.size(1) == rotary_dim / 2 && table.size(2) == 2,
+        "rotary: table must be (", (int64_t)llmt::kRopeTableRows, ", rotary_dim / 2, 2) float32");
+  auto shape = [&](const at::Tensor& x, const char* name) {
+    CHECK(x.dim() == 4 && x.size(0) == B && x.size(1) == T && x.size(3) == hd, "rotary: ", name, " must be (", B, ", ", T, ", heads, ", hd, ")");
+    CHECK(x.scalar_type() == q.scalar_type(), "rotary: q, k and their outputs must share a dtype");
+    CHECK(hd == 1 || x.stride(3) == 1 || x.numel() == 0, "rotary: ", name, " must have unit stride along head_dim");
+  };
+  auto fresh_or = [&](const c10::optional<at::Tensor>& given, const at::Tensor& x, const char* name) {
+    if (!(given.has_value() && given->defined())) return at::empty({B, T, x.size(2), hd}, x.options());
+    shape(*given, name);
+    CHECK(given->size(2) == x.size(2), "rotary: ", name, " has other heads than its input");
+    if (given->numel() > 0) {
+      // strides that step over one another's extent, smallest first
+      std::vector<std::pair<int64_t, int64_t>> d;
+      for (int i = 0; i < 3; ++i)
+        if (given->size(i) > 1) d.emplace_back(given->stride(i), given->size(i));
+      std::sort(d.begin(), d.end());
+      int64_t extent = hd;
+      for (auto& s : d) {
+        CHECK(s.first >= extent, "rotary: values of ", name, " overlap");
+        extent += s.first * (s.second - 1);
+      }
+      auto end = [&](const at::Tensor& t) {
+        int64_t e = hd;
+        for (int i = 0; i < 3; ++i) e += t.stride(i) * (t.size(i) - 1);
+        return (const char*)t.data_ptr() + e * t.element_size();
+      };
+      const bool same = given->data_ptr() == x.data_ptr() && given->strides() == x.strides();
+      CHECK(same || (const char*)given->data_ptr() >= end(x) || end(*given) <= (const char*)x.data_ptr(),
+            "rotary: ", name, " overlaps its input without being it");
+    }
+    return *given;
+  };
+  shape(q, "q");
+  if (has_k) shape(*k, "k");
+  CHECK(has_k || !k_out.has_value(), "rotary: k_out without k");
+  llmt::RopeArgs a{};
+  a.B = (int)B;
+  a.T = (int)T;
+  a.hd = (int)hd;
+  a.rd = (int)rotary_dim;
+  if (positions.has_value() && positions->defined()) {
+    CHECK(positions->scalar_type() == at::kInt || positions->scalar_type() == at::kLong, "rotary: positions must be int32 or int64");
+    CHECK(positions->dim() >= 1 && positions->dim() <= 2 && (positions->size(-1) == T || positions->size(-1) == 1) &&
+              (positions->dim() == 1 || positions->size(0) == B || positions->size(0) == 1),
+          "rotary: positions must be (", B, ", ", T, ") or broadcast to it");
+    a.pos = positions->data_ptr();
+    a.pos64 = positions->scalar_type() == at::kLong;
+    a.pst = positions->size(-1) == 1 ? 0 : positions->stride(-1);
+    a.psb = positions->dim() == 1 || positions->size(0) == 1 ? 0 : positions->stride(0);
+    if (T > 1 && positions->size(-1) == 1) CHECK(false, "rotary: one position for ", T, " tokens");
+  }
+  all_on_device({{q, "q"}, {k, "k"}, {positions, "positions"}, {table, "table"}, {q_out, "q_out"}, {k_out, "k_out"}});
+  at::Tensor qo = fresh_or(q_out, q, "q_out"), ko;
+  a.q = rope_heads(q, qo);
+  if (has_k) {
+    ko = fresh_or(k_out, *k, "k_out");
+    a.k = rope_heads(*k, ko);
+  }
+  a.table = table.data_ptr<float>();
+  a.interleaved = interleaved;
+  a.inverse = inverse;
+  if (B * T > 0) ok(llmt::rotary(a, kind, stream()), "rotary");
+  return {qo, ko};
+}
+
 // ---------------------------------------------------------------- optimizer
 void adamw_step(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v, c10::optional<at::Tensor> p16, at::Tensor lr,
                 at::Tensor step, double b1, double b2, double eps, double wd, double grad_scale, bool zero_grad,
@@ -176,6 +278,133 @@ void adamw_step(at::Tensor p, at::Tensor g, at::Tensor m, at::Tensor v, c10::opt
   ok(llmt::adamw_step(p.data_ptr<float>(), g.data_ptr<float>(), m.data_ptr<float>(), v.data_ptr<float>(), p16p,
                       p.numel(), lr.data_ptr<float>(), step.data_ptr<int>(), h, zero_grad, stream(), (int)max_blocks),
      "adamw_step");
+}
+
+// The tensors of a MultiAdamW: their sizes and places in the states are fixed, their addresses are
+// read at every step.
+struct MultiPlan {
+  std::vector<at::Tensor> p, p16;
+  std::vector<double> wd;
+  std::vector<int64_t> numel, first_block;
+  int64_t blocks = 0;
+
+  MultiPlan(std::vector<at::Tensor> p_, std::vector<at::Tensor> p16_, std::vector<double> wd_)
+      : p(std::move(p_)), p16(std::move(p16_)), wd(std::move(wd_)) {
+    CHECK(!p.empty(), "adamw: no tensors");
+    CHECK(p16.empty() || p16.size() == p.size(), "adamw: one bf16 copy per tensor, or none");
+    CHECK(wd.size() == p.size(), "adamw: one weight decay per tensor");
+    std::vector<std::pair<const char*, const char*>> spans;
+    for (size_t i = 0; i < p.size(); ++i) {
+      CHECK(p[i].scalar_type() == at::kFloat, "adamw: parameter ", i, " has dtype ", p[i].scalar_type(), ", expected Float");
+      CHECK(p[i].is_contiguous(), "adamw: parameter ", i, " must be contiguous");
+      CHECK(p[i].numel() > 0, "adamw: parameter ", i, " is empty");
+      if (!p16.empty()) {
+        CHECK(p16[i].scalar_type() == at::kBFloat16 && p16[i].is_contiguous() && p16[i].numel() == p[i].numel(),
+              "adamw: bf16 copy ", i, " must be contiguous bf16 of its parameter's size");
+        spans.emplace_back((const char*)p16[i].data_ptr(), (const char*)p16[i].data_ptr() + 2 * p16[i].numel());
+      }
+      spans.emplace_back((const char*)p[i].data_ptr(), (const char*)p[i].data_ptr() + 4 * p[i].numel());
+      numel.push_back(p[i].numel());
+      first_block.push_back(blocks);
+      blocks += (p[i].numel() + 255) / 256;
+    }
+    CHECK(blocks < 0x7fffffff, "adamw: more than 2^31 - 1 blocks of 256 values");
+    std::sort(spans.begin(), spans.end());
+    for (size_t i = 1; i < spans.size(); ++i) CHECK(spans[i].first >= spans[i - 1].second, "adamw: two tensors share memory");
+  }
+
+  // grads: one per tensor, None leaves that tensor and its states as they are.
+  int64_t step(const pybind11::list& grads, int64_t bits, at::Tensor m, at::Tensor v, c10::optional<at::Tensor> ms,
+               c10::optional<at::Tensor> vs, at::Tensor lr, at::Tensor step, at::Tensor ticket, double b1, double b2, double eps,
+               double grad_scale, c10::optional<at::Tensor> grad_scale_dev, int64_t seed, bool zero_grad) {
+    CHECK(grads.size() == p.size(), "adamw: ", grads.size(), " gradients for ", p.size(), " tensors");
+    CHECK(bits == 8 || bits == 32, "adamw: states have 8 or 32 bits");
+    std::vector<llmt::MultiTensor> t;
+    t.reserve(p.size());
+    bool any = false, bf16 = false;
+    int64_t elsewhere = -1;
+    const int dev = m.get_device();
+    for (size_t i = 0; i < p.size(); ++i) {
+      pybind11::handle h = grads[i];
+      if (h.is_none()) continue;
+      CHECK(THPVariable_Check(h.ptr()), "adamw: gradient ", i, " is not a tensor");
+      const at::Tensor& g = THPVariable_Unpack(h.ptr());
+      const bool half = g.scalar_type() == at::kBFloat16;
+      CHECK(half || g.scalar_type() == at::kFloat, "adamw: gradient ", i, " has dtype ", g.scalar_type(), ", expected Float or BFloat16");
+      CHECK(!any || half == bf16, "adamw: gradients of two dtypes in one step");
+      any = true;
+      bf16 = half;
+      CHECK(g.numel() == numel[i] && g.is_contiguous(), "adamw: gradient ", i, " must be contiguous with ", numel[i], " values");
+      CHECK(p[i].numel() == numel[i] && p[i].is_contiguous() && p[i].scalar_type() == at::kFloat, "adamw: parameter ", i, " changed its size, layout or type");
+      if (!(g.is_cuda() && p[i].is_cuda() && g.get_device() == dev && p[i].get_device() == dev)) elsewhere = (int64_t)i;
+      if (!p16.empty()) {
+        CHECK(p16[i].numel() == numel[i] && p16[i].is_contiguous() && p16[i].scalar_type() == at::kBFloat16, "adamw: bf16 copy ", i, " changed");
+        if (!(p16[i].is_cuda() && p16[i].get_device() == dev)) elsewhere = (int64_t)i;
+      }
+      t.push_back({static_cast<float*>(p[i].data_ptr()), g.data_ptr(), p16.empty() ? nullptr : p16[i].data_ptr(), numel[i],
+                   (int32_t)first_block[i], 0, (float)wd[i]});
+    }
+    const int64_t n = 256 * blocks;
+    const at::ScalarType dt_m = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat, dt_v = bits == 8 ? at::kByte : at::kFloat;
+    CHECK(m.scalar_type() == dt_m && v.scalar_type() == dt_v && m.numel() == n && v.numel() == n && m.is_contiguous() &&
+              v.is_contiguous(),
+          "adamw: states of another type or size");
+    if (bits == 8)
+      for (auto* x : {&ms, &vs})
+        CHECK(x->has_value() && (*x)->scalar_type() == at::kByte && (*x)->numel() == blocks && (*x)->is_contiguous(),
+              "adamw: one scale byte per block of 256 values");
+    CHECK(lr.scalar_type() == at::kFloat && step.scalar_type() == at::kInt && ticket.scalar_type() == at::kInt,
+          "adamw: lr must be float32, the step count and the ticket int32");
+    if (grad_scale_dev.has_value())
+      CHECK(grad_scale_dev->scalar_type() == at::kFloat && grad_scale_dev->numel() == 1, "adamw: grad_scale must be one float32 value");
+    for (auto* x : {&m, &v, &lr, &step, &ticket}) on_device(*x, "adamw state");
+    CHECK(elsewhere < 0, "adamw: tensor ", elsewhere, " is not on the states' device");
+    if (t.empty()) {
+      step.add_(1);
+      return 0;
+    }
+    llmt::MultiHyper h{(float)b1, (float)(1.0 - b1), (float)b2, (float)(1.0 - b2), (float)eps, (float)grad_scale,
+                       lr.data_ptr<float>(), static_cast<const float*>(opt_ptr(grad_scale_dev, "grad_scale")),
+                       step.data_ptr<int>(), reinterpret_cast<unsigned*>(ticket.data_ptr<int>()), (uint32_t)seed, zero_grad};
+    llmt::MultiState s{m.data_ptr(), v.data_ptr(), static_cast<uint8_t*>(const_cast<void*>(opt_ptr(ms, "scale"))),
+                       static_cast<uint8_t*>(const_cast<void*>(opt_ptr(vs, "scale")))};
+    ok(llmt::adamw_multi(t.data(), (int)t.size(), bf16, (int)bits, h, s, stream()), "adamw_multi");
+    return 1;
+  }
+};
+
+void check_codes(const at::Tensor& m, const at::Tensor& ms, const at::Tensor& v, const at::Tensor& vs) {
+  for (auto* t : {&m, &ms, &v, &vs}) {
+    CHECK(t->element_size() == 1 && t->is_contiguous(), "adamw: codes and scales are contiguous bytes");
+    on_device(*t, "adamw state");
+  }
+  CHECK(m.numel() == v.numel() && m.numel() == 256 * ms.numel() && ms.numel() == vs.numel(),
+        "adamw: one scale byte per block of 256 codes");
+}
+
+// (m, v) that the codes stand for, bf16 (exact) or fp32.
+std::vector<at::Tensor> adamw_state_values(at::Tensor m, at::Tensor ms, at::Tensor v, at::Tensor vs, bool f32) {
+  check_codes(m, ms, v, vs);
+  auto o = m.options().dtype(f32 ? at::kFloat : at::kBFloat16);
+  auto mo = at::empty(m.sizes(), o), vo = at::empty(v.sizes(), o);
+  ok(llmt::adamw_state_values(static_cast<const uint8_t*>(m.data_ptr()), static_cast<const uint8_t*>(ms.data_ptr()),
+                              static_cast<const uint8_t*>(v.data_ptr()), static_cast<const uint8_t*>(vs.data_ptr()),
+                              mo.data_ptr(), vo.data_ptr(), f32, m.numel(), stream()),
+     "adamw_state_values");
+  return {mo, vo};
+}
+
+void adamw_encode_states(at::Tensor m32, at::Tensor v32, at::Tensor m, at::Tensor ms, at::Tensor v, at::Tensor vs) {
+  check_codes(m, ms, v, vs);
+  for (auto* t : {&m32, &v32}) {
+    CHECK_DT((*t), at::kFloat);
+    CHECK(t->is_contiguous() && t->numel() == m.numel(), "adamw: fp32 states must be contiguous and match the codes");
+    on_device(*t, "adamw state");
+  }
+  ok(llmt::adamw_encode_states(m32.data_ptr<float>(), v32.data_ptr<float>(), static_cast<uint8_t*>(m.data_ptr()),
+                               static_cast<uint8_t*>(ms.data_ptr()), static_cast<uint8_t*>(v.data_ptr()),
+                               static_cast<uint8_t*>(vs.data_ptr()), ms.numel(), stream()),
+     "adamw_encode_states");
 }
 
 void cast_bf16(at::Tensor x, at::Tensor y, int64_t max_blocks) {
@@ -213,6 +442,278 @@ void ce_combine(at::Tensor part, at::Tensor tlogit, at::Tensor tgt, at::Tensor l
   ok(llmt::ce_combine(part.data_ptr<float>(), tlogit.data_ptr<float>(), tgt.data_ptr<int64_t>(), lse.data_ptr<float>(),
                       loss.data_ptr<float>(), (int)lse.numel(), (int)nblk, (int)V, stream()),
      "ce_combine");
+}
+
+// ---------------------------------------------------------------- post-training losses
+int float_kind(const at::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return 0;
+    case at::kHalf: return 1;
+    case at::kFloat: return 2;
+    default: CHECK(false, name, " has dtype ", t.scalar_type(), ", expected bfloat16, float16 or float32");
+  }
+  return -1;
+}
+
+// A (B, T) operand, broadcast where it has fewer or unit dimensions; empty when not given.
+template <typename E>
+llmt::Strided<E> strided_bt(const c10::optional<at::Tensor>& t, at::ScalarType dt, int64_t B, int64_t T, const char* name) {
+  if (!(t.has_value() && t->defined())) return {nullptr, 0, 0};
+  CHECK(t->scalar_type() == dt, name, " has dtype ", t->scalar_type(), ", expected ", dt);
+  CHECK(t->dim() <= 2, name, " must be (batch, tokens) or broadcast to it");
+  int64_t sb = 0, st = 0;
+  if (t->dim() >= 1) {
+    const int64_t n = t->size(-1);
+    CHECK(n == T || n == 1, name, " has ", n, " tokens, the logits ", T);
+    st = n == 1 ? 0 : t->stride(-1);
+  }
+  if (t->dim() == 2) {
+    CHECK(t->size(0) == B || t->size(0) == 1, name, " has ", t->size(0), " sequences, the logits ", B);
+    sb = t->size(0) == 1 ? 0 : t->stride(0);
+  }
+  return {static_cast<const E*>(t->data_ptr()), sb, st};
+}
+
+// Shapes and types are checked first, so that they are told apart from a tensor of another device.
+void all_on_device(std::initializer_list<std::pair<const c10::optional<at::Tensor>, const char*>> given) {
+  for (const auto& g : given)
+    if (g.first.has_value() && g.first->defined()) on_device(*g.first, g.second);
+}
+
+void no_grad_wanted(const c10::optional<at::Tensor>& t, const char* name) {
+  CHECK(!(t.has_value() && t->defined() && t->requires_grad()), name, " requires a gradient, which this loss does not give: detach it");
+}
+
+llmt::TokenBatch token_batch(const at::Tensor& targets, const c10::optional<at::Tensor>& mask, int64_t B, int64_t T, int64_t V) {
+  CHECK(B > 0 && T > 0, "empty batch (", B, " sequences of ", T, " tokens)");
+  CHECK(V > 0 && V < (int64_t(1) << 30), "a vocabulary of ", V, " ids");
+  CHECK(B * T <= 0x7fffffff, "more than 2^31 - 1 tokens");
+  CHECK(targets.dim() == 2 && targets.size(0) == B && targets.size(1) == T, "targets must be (", B, ", ", T, ")");
+  llmt::TokenBatch a{};
+  a.B = (int)B;
+  a.T = (int)T;
+  a.V = (int)V;
+  a.tgt = strided_bt<int64_t>(targets, at::kLong, B, T, "targets");
+  a.mask = strided_bt<uint8_t>(mask, at::kBool, B, T, "mask");
+  return a;
+}
+
+llmt::TokenBatch logit_batch(const at::Tensor& logits, const at::Tensor& targets, const c10::optional<at::Tensor>& mask) {
+  CHECK(logits.dim() == 3, "logits must be (batch, tokens, vocabulary)");
+  llmt::TokenBatch a = token_batch(targets, mask, logits.size(0), logits.size(1), logits.size(2));
+  CHECK(logits.stride(2) == 1 || logits.size(2) == 1, "logits must have unit stride along the vocabulary");
+  a.dtype = float_kind(logits, "logits");
+  a.z = logits.data_ptr();
+  a.zsb = logits.stride(0);
+  a.zst = logits.stride(1);
+  return a;
+}
+
+// The rows written to: `out`, or a new contiguous tensor. Rows of `out` may not overlap one
+// another; `out` may be the logits themselves, but not other rows of theirs.
+at::Tensor gradient_rows(const at::Tensor& logits, const c10::optional<at::Tensor>& out, llmt::RowOut& o) {
+  at::Tensor d;
+  if (out.has_value() && out->defined()) {
+    d = *out;
+    CHECK(d.scalar_type() == logits.scalar_type() && d.sizes() == logits.sizes(), "out must match the logits");
+    const int64_t B = d.size(0), T = d.size(1), V = d.size(2), sb = d.stride(0), st = d.stride(1);
+    CHECK(d.stride(2) == 1 || V == 1, "out must have unit stride along the vocabulary");
+    const bool rows_in = T == 1 || (st >= V && (B == 1 || sb >= (T - 1) * st + V));
+    const bool rows_out = B == 1 || (sb >= V && (T == 1 || st >= (B - 1) * sb + V));
+    CHECK(rows_in || rows_out, "rows of out overlap");
+    const bool same = d.data_ptr() == logits.data_ptr() && d.strides() == logits.strides();
+    const int64_t e = d.element_size();
+    auto last = [&](const at::Tensor& t) {
+      return (const char*)t.data_ptr() + e * ((B - 1) * t.stride(0) + (T - 1) * t.stride(1) + V);
+    };
+    CHECK(same || (const char*)d.data_ptr() >= last(logits) || last(d) <= (const char*)logits.data_ptr(),
+          "out overlaps the logits without being the same rows");
+  } else {
+    d = at::empty(logits.sizes(), logits.options());
+  }
+  o.dz = d.data_ptr();
+  o.sb = d.stride(0);
+  o.st = d.stride(1);
+  return d;
+}
+
+const float* grad_scalar(const c10::optional<at::Tensor>& g) {
+  if (!(g.has_value() && g->defined())) return nullptr;
+  CHECK(g->scalar_type() == at::kFloat && g->numel() == 1, "grad_out must be one float32 value");
+  return g->data_ptr<float>();
+}
+
+// (logp (B, T), stats (B, T, 2)) of rows of logits.
+std::vector<at::Tensor> logprob_rows(at::Tensor logits, at::Tensor targets, c10::optional<at::Tensor> mask) {
+  llmt::TokenBatch a = logit_batch(logits, targets, mask);
+  all_on_device({{logits, "logits"}, {targets, "targets"}, {mask, "mask"}});
+  auto f = logits.options().dtype(at::kFloat);
+  auto logp = at::empty({a.B, a.T}, f), stats = at::empty({a.B, a.T, 2}, f);
+  llmt::RowOut o{};
+  o.logp = logp.data_ptr<float>();
+  o.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
+  ok(llmt::logprob_rows(a, o, stream()), "logprob_rows");
+  return {logp, stats};
+}
+
+llmt::PolicyArgs policy_args(const c10::optional<at::Tensor>& old, const at::Tensor& adv, const c10::optional<at::Tensor>& ref,
+                             int64_t B, int64_t T, double clip_lo, double clip_hi, double kl, int64_t reduction) {
+  no_grad_wanted(old, "old_logp");
+  no_grad_wanted(adv, "advantages");
+  no_grad_wanted(ref, "ref_logp");
+  CHECK(clip_lo >= 0 && clip_lo <= 1 && clip_hi >= 0, "clip must be (low in [0, 1], high >= 0)");
+  CHECK(reduction >= 0 && reduction <= 2, "unknown reduction");
+  llmt::PolicyArgs q{};
+  q.old = strided_bt<float>(old, at::kFloat, B, T, "old_logp");
+  q.adv = strided_bt<float>(adv, at::kFloat, B, T, "advantages");
+  q.ref = strided_bt<float>(ref, at::kFloat, B, T, "ref_logp");
+  q.clip_lo = (float)clip_lo;
+  q.clip_hi = (float)clip_hi;
+  q.kl_coef = (float)kl;
+  q.reduction = (int)reduction;
+  return q;
+}
+
+// (loss, logp, coef, stats, dlogits): dlogits undefined unless `grad`.
+std::vector<at::Tensor> policy_rows(at::Tensor logits, at::Tensor targets, c10::optional<at::Tensor> old, at::Tensor adv,
+                                    c10::optional<at::Tensor> ref, c10::optional<at::Tensor> mask, double clip_lo,
+                                    double clip_hi, double kl, int64_t reduction, bool grad,
+                                    c10::optional<at::Tensor> out) {
+  llmt::TokenBatch a = logit_batch(logits, targets, mask);
+  const llmt::PolicyArgs q = policy_args(old, adv, ref, a.B, a.T, clip_lo, clip_hi, kl, reduction);
+  llmt::RowOut o{};
+  at::Tensor d;
+  if (grad && out.has_value()) d = gradient_rows(logits, out, o);
+  all_on_device({{logits, "logits"}, {targets, "targets"}, {mask, "mask"}, {old, "old_logp"}, {adv, "advantages"},
+                 {ref, "ref_logp"}, {out, "out"}});
+  if (grad && !d.defined()) d = gradient_rows(logits, out, o);
+  auto f = logits.options().dtype(at::kFloat);
+  const int64_t n = (int64_t)a.B * a.T;
+  auto loss = at::empty({}, f), logp = at::empty({a.B, a.T}, f), coef = at::empty({a.B, a.T}, f),
+       stats = at::empty({a.B, a.T, 2}, f), rows = at::empty({n}, f), words = at::empty({a.B + 1}, f.dtype(at::kInt));
+  o.logp = logp.data_ptr<float>();
+  o.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
+  o.loss = loss.data_ptr<float>();
+  o.loss_rows = rows.data_ptr<float>();
+  o.coef = coef.data_ptr<float>();
+  o.count = words.data_ptr<int>();
+  o.ticket = reinterpret_cast<unsigned*>(o.count + a.B);
+  ok(llmt::policy_rows(a, q, o, stream()), "policy_rows");
+  return {loss, logp, coef, stats, d};
+}
+
+// (loss, coef) of log-probabilities.
+std::vector<at::Tensor> policy_tokens(at::Tensor logp, at::Tensor targets, int64_t V, c10::optional<at::Tensor> old,
+                                      at::Tensor adv, c10::optional<at::Tensor> ref, c10::optional<at::Tensor> mask,
+                                      double clip_lo, double clip_hi, double kl, int64_t reduction) {
+  CHECK_DT(logp, at::kFloat);
+  CHECK(logp.dim() == 2 && logp.is_contiguous(), "logp must be a contiguous (batch, tokens) tensor");
+  llmt::TokenBatch a = token_batch(targets, mask, logp.size(0), logp.size(1), V);
+  const llmt::PolicyArgs q = policy_args(old, adv, ref, a.B, a.T, clip_lo, clip_hi, kl, reduction);
+  all_on_device({{logp, "logp"}, {targets, "targets"}, {mask, "mask"}, {old, "old_logp"}, {adv, "advantages"},
+                 {ref, "ref_logp"}});
+  auto f = logp.options();
+  auto loss = at::empty({}, f), coef = at::empty({a.B, a.T}, f), rows = at::empty({(int64_t)a.B * a.T}, f),
+       words = at::empty({a.B + 1}, f.dtype(at::kInt));
+  llmt::RowOut o{};
+  o.loss = loss.data_ptr<float>();
+  o.loss_rows = rows.data_ptr<float>();
+  o.coef = coef.data_ptr<float>();
+  o.count = words.data_ptr<int>();
+  o.ticket = reinterpret_cast<unsigned*>(o.count + a.B);
+  ok(llmt::policy_tokens(a, q, logp.data_ptr<float>(), o, stream()), "policy_tokens");
+  return {loss, coef};
+}
+
+llmt::PreferenceArgs preference_args(const c10::optional<at::Tensor>& ref, int64_t B, int64_t T, double beta,
+                                     double smoothing, int64_t kind, bool average) {
+  no_grad_wanted(ref, "ref_logp");
+  CHECK(B % 2 == 0, "the batch holds the chosen sequences, then as many rejected ones: got ", B);
+  CHECK(beta > 0, "beta must be positive");
+  CHECK(smoothing >= 0 && smoothing < 0.5, "label_smoothing must be in [0, 0.5)");
+  CHECK(kind >= 0 && kind <= 2, "unknown preference loss");
+  CHECK(smoothing == 0 || kind == llmt::PREF_SIGMOID, "label_smoothing goes with the sigmoid loss");
+  llmt::PreferenceArgs q{};
+  q.ref = strided_bt<float>(ref, at::kFloat, B, T, "ref_logp");
+  q.beta = (float)beta;
+  q.smoothing = (float)smoothing;
+  q.kind = (int)kind;
+  q.average = average;
+  return q;
+}
+
+std::vector<at::Tensor> preference_parts(const llmt::TokenBatch& a, const llmt::PreferenceArgs& q, const at::Tensor& logp,
+                                         const at::Tensor& ticket, bool ready, llmt::RowOut& o) {
+  auto f = logp.options();
+  auto loss = at::empty({}, f), coef = at::empty({a.B, a.T}, f), rewards = at::empty({a.B}, f),
+       rows = at::empty({a.B / 2}, f);
+  o.loss = loss.data_ptr<float>();
+  o.loss_rows = rows.data_ptr<float>();
+  o.coef = coef.data_ptr<float>();
+  o.rewards = rewards.data_ptr<float>();
+  o.ticket = reinterpret_cast<unsigned*>(ticket.data_ptr<int>());
+  ok(llmt::preference_tokens(a, q, logp.data_ptr<float>(), o, ready, stream()), "preference_tokens");
+  return {loss, coef, rewards};
+}
+
+// (loss, logp, rewards, coef, stats, dlogits): dlogits undefined unless `grad`.
+std::vector<at::Tensor> preference_rows(at::Tensor logits, at::Tensor targets, c10::optional<at::Tensor> ref,
+                                        c10::optional<at::Tensor> mask, double beta, double smoothing, int64_t kind,
+                                        bool average, bool grad, c10::optional<at::Tensor> out) {
+  llmt::TokenBatch a = logit_batch(logits, targets, mask);
+  const llmt::PreferenceArgs q = preference_args(ref, a.B, a.T, beta, smoothing, kind, average);
+  llmt::RowOut o{};
+  at::Tensor d;
+  if (grad && out.has_value()) d = gradient_rows(logits, out, o);
+  all_on_device({{logits, "logits"}, {targets, "targets"}, {mask, "mask"}, {ref, "ref_logp"}, {out, "out"}});
+  if (grad && !d.defined()) d = gradient_rows(logits, out, o);
+  auto f = logits.options().dtype(at::kFloat);
+  auto logp = at::empty({a.B, a.T}, f), stats = at::empty({a.B, a.T, 2}, f), ticket = at::empty({1}, f.dtype(at::kInt));
+  o.logp = logp.data_ptr<float>();
+  o.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
+  o.ticket = reinterpret_cast<unsigned*>(ticket.data_ptr<int>());
+  llmt::RowOut first = o;
+  first.dz = nullptr;
+  ok(llmt::logprob_rows(a, first, stream()), "preference_rows");
+  auto r = preference_parts(a, q, logp, ticket, true, o);
+  if (grad) ok(llmt::grad_rows(a, o, false, stream()), "preference_rows");
+  return {r[0], logp, r[2], r[1], stats, d};
+}
+
+// (loss, coef, rewards) of log-probabilities.
+std::vector<at::Tensor> preference_tokens(at::Tensor logp, at::Tensor targets, int64_t V, c10::optional<at::Tensor> ref,
+                                          c10::optional<at::Tensor> mask, double beta, double smoothing, int64_t kind,
+                                          bool average) {
+  CHECK_DT(logp, at::kFloat);
+  CHECK(logp.dim() == 2 && logp.is_contiguous(), "logp must be a contiguous (batch, tokens) tensor");
+  llmt::TokenBatch a = token_batch(targets, mask, logp.size(0), logp.size(1), V);
+  const llmt::PreferenceArgs q = preference_args(ref, a.B, a.T, beta, smoothing, kind, average);
+  all_on_device({{logp, "logp"}, {targets, "targets"}, {mask, "mask"}, {ref, "ref_logp"}});
+  auto ticket = at::empty({1}, logp.options().dtype(at::kInt));
+  llmt::RowOut o{};
+  return preference_parts(a, q, logp, ticket, false, o);
+}
+
+// Gradient rows coef (onehot - softmax) * grad_out from saved stats; with skip_one `out` holds
+// them already where grad_out is 1.
+at::Tensor grad_rows(at::Tensor logits, at::Tensor targets, c10::optional<at::Tensor> mask, at::Tensor coef,
+                     at::Tensor stats, c10::optional<at::Tensor> grad_out, c10::optional<at::Tensor> out, bool skip_one) {
+  llmt::TokenBatch a = logit_batch(logits, targets, mask);
+  const int64_t n = (int64_t)a.B * a.T;
+  for (auto* t : {&coef, &stats}) {
+    CHECK_DT((*t), at::kFloat);
+    CHECK(t->is_contiguous() && t->numel() == (t == &coef ? n : 2 * n), "grad_rows: coef (batch, tokens), stats (batch, tokens, 2)");
+  }
+  const float* g = grad_scalar(grad_out);
+  llmt::RowOut o{};
+  all_on_device({{logits, "logits"}, {targets, "targets"}, {mask, "mask"}, {coef, "coef"}, {stats, "stats"},
+                 {grad_out, "grad_out"}, {out, "out"}});
+  at::Tensor d = gradient_rows(logits, out, o);
+  o.coef = coef.data_ptr<float>();
+  o.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
+  o.grad_out = g;
+  ok(llmt::grad_rows(a, o, skip_one, stream()), "grad_rows");
+  return d;
 }
 
 // ---------------------------------------------------------------- fp8 quantization
@@ -570,6 +1071,26 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_fwd_rows", &ce_fwd_rows);
   m.def("ce_bwd_rows", &ce_bwd_rows);
   m.def("ce_combine", &ce_combine);
+  py::class_<MultiPlan>(m, "MultiPlan")
+      .def(py::init<std::vector<at::Tensor>, std::vector<at::Tensor>, std::vector<double>>(), "p"_a, "p16"_a, "wd"_a)
+      .def_readonly("blocks", &MultiPlan::blocks)
+      .def_readonly("first_block", &MultiPlan::first_block)
+      .def("step", &MultiPlan::step);
+  m.def("adamw_state_values", &adamw_state_values, "m"_a, "ms"_a, "v"_a, "vs"_a, "f32"_a = false);
+  m.def("adamw_encode_states", &adamw_encode_states, "m32"_a, "v32"_a, "m"_a, "ms"_a, "v"_a, "vs"_a);
+  m.def("rotary", &rotary, "q"_a, "k"_a, "positions"_a, "table"_a, "rotary_dim"_a, "interleaved"_a, "inverse"_a,
+        "q_out"_a = py::none(), "k_out"_a = py::none());
+  m.def("logprob_rows", &logprob_rows, "logits"_a, "targets"_a, "mask"_a = py::none());
+  m.def("policy_rows", &policy_rows, "logits"_a, "targets"_a, "old"_a, "adv"_a, "ref"_a, "mask"_a, "clip_lo"_a,
+        "clip_hi"_a, "kl"_a, "reduction"_a, "grad"_a, "out"_a = py::none());
+  m.def("policy_tokens", &policy_tokens, "logp"_a, "targets"_a, "V"_a, "old"_a, "adv"_a, "ref"_a, "mask"_a, "clip_lo"_a,
+        "clip_hi"_a, "kl"_a, "reduction"_a);
+  m.def("preference_rows", &preference_rows, "logits"_a, "targets"_a, "ref"_a, "mask"_a, "beta"_a, "smoothing"_a,
+        "kind"_a, "average"_a, "grad"_a, "out"_a = py::none());
+  m.def("preference_tokens", &preference_tokens, "logp"_a, "targets"_a, "V"_a, "ref"_a, "mask"_a, "beta"_a, "smoothing"_a,
+        "kind"_a, "average"_a);
+  m.def("grad_rows", &grad_rows, "logits"_a, "targets"_a, "mask"_a, "coef"_a, "stats"_a, "grad_out"_a = py::none(),
+        "out"_a = py::none(), "skip_one"_a = false);
   m.def("gemm", &gemm, "a"_a, "b"_a, "ta"_a, "tb"_a, "epi"_a, "out"_a, "accumulate"_a = false, "aux"_a = py::none(),
         "out2"_a = py::none(), "split"_a = 0, "cos_t"_a = py::none(), "sin_t"_a = py::none(), "T"_a = 0, "hd"_a = 0,
         "rot_cols"_a = 0, "tgt"_a = py::none(), "lse"_a = py::none(), "grad_out"_a = py::none(), "part"_a = py::none(),

@@ -130,7 +130,7 @@ struct Strided {
 struct TokenBatch {
   const void* z;
   int dtype, B, T, V;
-  int64_t zsb, zst;
+  int64_t zsb, zst, zn;  // element strides, and the elements from the first to the last
   Strided<int64_t> tgt;
   Strided<uint8_t> mask;
 };
@@ -157,17 +157,20 @@ struct RowOut {
   int* count;        // (B) scratch of the policy loss
   unsigned* ticket;  // (1) scratch
   void* dz;          // gradient rows, the logits' type, or nullptr; may be z itself
-  int64_t sb, st;    // their element strides
+  int64_t sb, st, dn;  // their element strides, and the elements from the first to the last
   const float* grad_out;  // device scalar that multiplies the gradient, or nullptr
 };
 cudaError_t logprob_rows(const TokenBatch& a, const RowOut& o, cudaStream_t st);
 cudaError_t policy_rows(const TokenBatch& a, const PolicyArgs& q, const RowOut& o, cudaStream_t st);
 cudaError_t policy_tokens(const TokenBatch& a, const PolicyArgs& q, const float* logp, const RowOut& o, cudaStream_t st);
-// ticket_ready: the ticket is zero already (logprob_rows leaves it so), else it is cleared here.
+// ticket_ready: called right after logprob_rows with the same o, which leaves the ticket zero; else it
+// is cleared here.
 cudaError_t preference_tokens(const TokenBatch& a, const PreferenceArgs& q, const float* logp, const RowOut& o,
                               bool ticket_ready, cudaStream_t st);
-// dz from coef and stats; skip_one: dz holds it already where *grad_out is 1.
-cudaError_t grad_rows(const TokenBatch& a, const RowOut& o, bool skip_one, cudaStream_t st);
+// dz from coef and stats; skip_one: dz holds it already where *grad_out is 1; after_loss: called right
+// after preference_tokens, which wrote coef.
+cudaError_t grad_rows(const TokenBatch& a, const RowOut& o, bool skip_one, bool after_loss, cudaStream_t st);
+int loss_error_code(bool reset);
 
 // ---------------------------------------------------------------- GEMM
 enum EpiKind : int {

@@ -506,6 +506,7 @@ llmt::TokenBatch logit_batch(const at::Tensor& logits, const at::Tensor& targets
   a.z = logits.data_ptr();
   a.zsb = logits.stride(0);
   a.zst = logits.stride(1);
+  a.zn = (logits.size(0) - 1) * a.zsb + (logits.size(1) - 1) * a.zst + a.V;
   return a;
 }
 
@@ -534,6 +535,7 @@ at::Tensor gradient_rows(const at::Tensor& logits, const c10::optional<at::Tenso
   o.dz = d.data_ptr();
   o.sb = d.stride(0);
   o.st = d.stride(1);
+  o.dn = (d.size(0) - 1) * o.sb + (d.size(1) - 1) * o.st + d.size(2);
   return d;
 }
 
@@ -676,7 +678,7 @@ std::vector<at::Tensor> preference_rows(at::Tensor logits, at::Tensor targets, c
   first.dz = nullptr;
   ok(llmt::logprob_rows(a, first, stream()), "preference_rows");
   auto r = preference_parts(a, q, logp, ticket, true, o);
-  if (grad) ok(llmt::grad_rows(a, o, false, stream()), "preference_rows");
+  if (grad) ok(llmt::grad_rows(a, o, false, true, stream()), "preference_rows");
   return {r[0], logp, r[2], r[1], stats, d};
 }
 
@@ -712,7 +714,7 @@ at::Tensor grad_rows(at::Tensor logits, at::Tensor targets, c10::optional<at::Te
   o.coef = coef.data_ptr<float>();
   o.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
   o.grad_out = g;
-  ok(llmt::grad_rows(a, o, skip_one, stream()), "grad_rows");
+  ok(llmt::grad_rows(a, o, skip_one, false, stream()), "grad_rows");
   return d;
 }
 
@@ -1080,6 +1082,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adamw_encode_states", &adamw_encode_states, "m32"_a, "v32"_a, "m"_a, "ms"_a, "v"_a, "vs"_a);
   m.def("rotary", &rotary, "q"_a, "k"_a, "positions"_a, "table"_a, "rotary_dim"_a, "interleaved"_a, "inverse"_a,
         "q_out"_a = py::none(), "k_out"_a = py::none());
+  m.def("loss_error_code", &llmt::loss_error_code, "reset"_a = false);
   m.def("logprob_rows", &logprob_rows, "logits"_a, "targets"_a, "mask"_a = py::none());
   m.def("policy_rows", &policy_rows, "logits"_a, "targets"_a, "old"_a, "adv"_a, "ref"_a, "mask"_a, "clip_lo"_a,
         "clip_hi"_a, "kl"_a, "reduction"_a, "grad"_a, "out"_a = py::none());

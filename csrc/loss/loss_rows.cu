@@ -15,27 +15,47 @@
 // A token counts where its mask is set and its target is an id of the vocabulary; the logits of
 // every other row are not read (they may hold anything), and its gradient is zero.
 //
-// Each row is summed by one CTA; sums, maxima and slopes are fp32, the sums over tokens fp64, and
-// the gradient is rounded once, to the logits' type. No atomics touch a result: equal inputs give
-// equal bits.
+// A row is held in the shared memory of a cluster of 1 to 8 CTAs, each a run of its 16-byte pieces: the
+// logits are read once, the maximum and sum of each warp are exchanged through distributed shared
+// memory, and the gradient is computed from what is held. Rows that do not fit (over 512 KB) are
+// read again. Sums, maxima and slopes are fp32, the sums over tokens fp64, and the gradient is
+// rounded once, to the logits' type. No atomics touch a result: equal inputs give equal bits.
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "../common/common.cuh"
+#include "../common/sm100.cuh"
 
 namespace llmt {
 namespace {
 
-constexpr int kRowThreads = 512;
+constexpr int kMaxThreads = 256;        // of a CTA of a row: with 512, the 40 registers left to each cost 13%
+constexpr int kSliceBytes = 64 * 1024;  // of a row in a CTA's shared memory: three CTAs a SM
+constexpr int kMaxCluster = 8;
 constexpr int kPairThreads = 256;
 
-// e^x through the exponential of two. log2(e) in one fp32 number is 1.3e-8 short, which makes every
-// e^-8 of a row's sum 1e-7 too large: a bias that the sum of a long sequence's log-probabilities
-// shows (3.8e-5 of a reward over 700 tokens; 7e-6 with the second part of the constant).
+// Exponentials. Errors of one sign matter here: those of 700 tokens' log-probabilities add up in the
+// reward of their sequence. log2(e) in one fp32 number is 1.3e-8 short, which makes an e^-8 1e-7 too large:
+// it has a second part below. The exponential of two is up to 8e-7 off and 5e-8 short in the mean
+// (measured on 2^20 arguments each in [-4 k - 4, -4 k], k = 0 .. 4: 4.5e-8 to 5.1e-8), which a row's
+// logarithm takes back (kShort); splitting the integer off first, as exp_ does for the few terms that join
+// sums, leaves 1e-8 but took a third of the kernel's instructions.
+constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596299e-8f;
+constexpr double kShort = 5e-8;
+// e^x for x <= 0; e^-87 below that.
 __device__ __forceinline__ float exp_(float x) {
-  const float t = fmaf(x, 1.44269502f, x * 1.92596299e-8f);
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t));
-  return y;
+  x = fmaxf(x, -87.f);
+  const float magic = 12582912.f;  // 1.5 2^23: adding it leaves the integer in the low bits
+  const float t = fmaf(x, kLog2e, magic);
+  const float f = fmaf(x, kLog2eLow, fmaf(x, kLog2e, magic - t));
+  return __uint_as_float(__float_as_uint(sm100::ex2_approx(f)) + (__float_as_uint(t) << 23));
+}
+// sum + e^(z - at), two values at a time.
+__device__ __forceinline__ float2 add_exp(float2 z, float2 minus_at, float2 sum) {
+  const float2 x = sm100::add2(z, minus_at);
+  const float2 t = sm100::fma2(x, make_float2(kLog2e, kLog2e), sm100::mul2(x, make_float2(kLog2eLow, kLog2eLow)));
+  return sm100::add2(sum, make_float2(sm100::ex2_approx(t.x), sm100::ex2_approx(t.y)));
 }
 
 // ---------------------------------------------------------------- 16-byte pieces of a row
@@ -52,44 +72,104 @@ __device__ __forceinline__ bf16 from_f<bf16>(float v) { return __float2bfloat16_
 template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 
+// 16 bytes of a row in registers: N values of T, in pairs.
 template <typename T>
-struct alignas(16) Piece {
+struct Piece {
   static constexpr int N = 16 / sizeof(T);
-  T v[N];
+  uint32_t u[4];
 };
+template <typename T>
+__device__ __forceinline__ float2 pair_of(const Piece<T>& x, int i) {
+  if constexpr (sizeof(T) == 4) {
+    return make_float2(__uint_as_float(x.u[2 * i]), __uint_as_float(x.u[2 * i + 1]));
+  } else if constexpr (std::is_same_v<T, bf16>) {
+    return make_float2(__uint_as_float(x.u[i] << 16), __uint_as_float(x.u[i] & 0xffff0000u));
+  } else {
+    const uint32_t u = x.u[i];
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+  }
+}
+template <typename T>
+__device__ __forceinline__ void put_pair(Piece<T>& x, int i, float2 f) {
+  if constexpr (sizeof(T) == 4) {
+    x.u[2 * i] = __float_as_uint(f.x);
+    x.u[2 * i + 1] = __float_as_uint(f.y);
+  } else if constexpr (std::is_same_v<T, bf16>) {
+    x.u[i] = pack_bf16x2(f.x, f.y);
+  } else {
+    const __half2 h = __floats2half2_rn(f.x, f.y);
+    x.u[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+// Larger of two values, NaN where either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (std::is_same_v<T, bf16>) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float piece_max(const Piece<T>& x, float m) {
+  if constexpr (sizeof(T) == 4) {
+    const float2 p = pair_of(x, 0), q = pair_of(x, 1);
+    return max_nan(m, max_nan(max_nan(p.x, p.y), max_nan(q.x, q.y)));
+  } else {
+    Piece<T> r;
+    r.u[0] = max2_nan<T>(max2_nan<T>(x.u[0], x.u[1]), max2_nan<T>(x.u[2], x.u[3]));
+    const float2 p = pair_of(r, 0);
+    return max_nan(m, max_nan(p.x, p.y));
+  }
+}
 
 // A row seen as 16-byte pieces at aligned addresses: piece c holds elements [c N - off, c N - off + N),
-// the first and the last one perhaps only in part.
+// the first and the last one perhaps only in part. at and n: the row's first element and the number of
+// elements of the buffer (the bounds-checked build's extents).
 template <typename T>
 struct RowView {
   static constexpr int N = Piece<T>::N;
   T* p;
-  int V, off, pieces;
-  __device__ RowView(T* row, int v) : p(row), V(v) {
-    off = (int)(((uintptr_t)row & 15) / sizeof(T));
+  int V, off, pieces, whole_lo, whole_hi;
+  int64_t at, n;
+  __device__ RowView(T* base, int64_t at_, int64_t n_, int v) : p(base + at_), V(v), at(at_), n(n_) {
+    off = (int)(((uintptr_t)p & 15) / sizeof(T));
     pieces = (off + v + N - 1) / N;
+    whole_lo = off ? 1 : 0;
+    whole_hi = (off + v) / N;
   }
-  __device__ __forceinline__ bool whole(int c) const { return c * N >= off && (c + 1) * N - off <= V; }
-  __device__ __forceinline__ Piece<T> load(int c) const {
-    const int e0 = c * N - off;
-    if (whole(c)) return *reinterpret_cast<const Piece<T>*>(p + e0);
-    Piece<T> r;
-#pragma unroll
-    for (int j = 0; j < N; ++j) r.v[j] = (e0 + j >= 0 && e0 + j < V) ? p[e0 + j] : from_f<T>(-INFINITY);
-    return r;
+  // Address of piece c (of whole pieces only, or to compare).
+  __device__ __forceinline__ uint4* piece(int c) const { return reinterpret_cast<uint4*>(p + ((int64_t)c * N - off)); }
+  // The element of place e of piece c, where the row has it.
+  __device__ __forceinline__ bool has(int c, int e) const {
+    const int i = c * N - off + e;
+    return i >= 0 && i < V && LLMT_IN(at + i, at + i + 1, n, 602);
   }
-  // Stores the piece that `like` (another view of as many elements) has at c.
-  __device__ __forceinline__ void store(const RowView& like, int c, const Piece<T>& x) const {
-    const int e0 = c * N - like.off;
-    if (like.off == off && whole(c)) {
-      *reinterpret_cast<Piece<T>*>(p + e0) = x;
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (e0 + j >= 0 && e0 + j < V) p[e0 + j] = x.v[j];
-  }
+  __device__ __forceinline__ T& element(int c, int e) const { return p[(int64_t)c * N - off + e]; }
 };
+
+// The pieces of a row's ends, element by element; the missing ones are of -inf.
+template <typename T>
+__device__ uint4 load_part(const RowView<T>& r, int c) {
+  Piece<T> x;
+  for (int j = 0; j < Piece<T>::N / 2; ++j)
+    put_pair(x, j, make_float2(r.has(c, 2 * j) ? to_f(r.element(c, 2 * j)) : -INFINITY,
+                               r.has(c, 2 * j + 1) ? to_f(r.element(c, 2 * j + 1)) : -INFINITY));
+  return make_uint4(x.u[0], x.u[1], x.u[2], x.u[3]);
+}
+// Stores x, the piece c of a row that `like` views, into another view of it, element by element.
+template <typename T>
+__device__ void store_part(const RowView<T>& out, const RowView<T>& like, int c, const Piece<T>& x) {
+  for (int j = 0; j < Piece<T>::N; ++j) {
+    const int i = c * Piece<T>::N - like.off + j;
+    const float2 f = pair_of(x, j / 2);  // back to the type it came from: exact
+    if (i >= 0 && i < out.V && LLMT_IN(out.at + i, out.at + i + 1, out.n, 604)) out.p[i] = from_f<T>(j & 1 ? f.y : f.x);
+  }
+}
 
 // ---------------------------------------------------------------- tokens
 __device__ __forceinline__ bool token_counts(const TokenBatch& a, int b, int t, int64_t* y) {
@@ -103,6 +183,7 @@ __global__ void __launch_bounds__(256) count_tokens_kernel(TokenBatch a, int* co
   const int b = blockIdx.x;
   int n = 0;
   int64_t y;
+  pdl_trigger();
   for (int t = threadIdx.x; t < a.T; t += blockDim.x) n += token_counts(a, b, t, &y) ? 1 : 0;
   n = __reduce_add_sync(0xffffffffu, n);
   __shared__ int part[8];
@@ -115,40 +196,43 @@ __global__ void __launch_bounds__(256) count_tokens_kernel(TokenBatch a, int* co
   }
 }
 
-// Weight of a token of sequence b: the whole CTA calls it (it sums the counts of all sequences).
+// Weight of a token of sequence b, by one warp (it sums the counts of all sequences).
 __device__ __forceinline__ float token_weight(const int* count, int B, int b, int reduction) {
   if (reduction == LOSS_SUM) return 1.f;
-  __shared__ int s_sum, s_full;
-  if (threadIdx.x < 32) {
-    int sum = 0, full = 0;
-    for (int i = threadIdx.x; i < B; i += 32) {
-      sum += count[i];
-      full += count[i] > 0 ? 1 : 0;
-    }
-    sum = __reduce_add_sync(0xffffffffu, sum);
-    full = __reduce_add_sync(0xffffffffu, full);
-    if (threadIdx.x == 0) {
-      s_sum = sum;
-      s_full = full;
-    }
+  int sum = 0, full = 0;
+  for (int i = threadIdx.x & 31; i < B; i += 32) {
+    const int c = count[i];
+    sum += c;
+    full += c > 0 ? 1 : 0;
   }
-  __syncthreads();
-  if (reduction == LOSS_TOKEN) return 1.f / (float)s_sum;
-  return 1.f / ((float)count[b] * (float)s_full);
+  sum = __reduce_add_sync(0xffffffffu, sum);
+  if (reduction == LOSS_TOKEN) return 1.f / (float)sum;
+  full = __reduce_add_sync(0xffffffffu, full);
+  return 1.f / ((float)count[b] * (float)full);
+}
+
+// What the policy loss reads of one token.
+struct PolicyToken {
+  float adv, old, ref;
+};
+__device__ __forceinline__ PolicyToken load_token(const PolicyArgs& q, int b, int t) {
+  PolicyToken k;
+  k.adv = q.adv.p[b * q.adv.sb + t * q.adv.st];
+  k.old = q.old.p ? q.old.p[b * q.old.sb + t * q.old.st] : 0.f;
+  k.ref = q.ref.p ? q.ref.p[b * q.ref.sb + t * q.ref.st] : 0.f;
+  return k;
 }
 
 // Loss and slope of one token, both with the weight in.
-__device__ __forceinline__ void policy_token(const PolicyArgs& q, int b, int t, float logp, float w, float* loss,
+__device__ __forceinline__ void policy_token(const PolicyArgs& q, PolicyToken k, float logp, float w, float* loss,
                                              float* slope) {
-  const float A = q.adv.p[b * q.adv.sb + t * q.adv.st];
-  const float old = q.old.p ? q.old.p[b * q.old.sb + t * q.old.st] : logp;
-  const float r = expf(logp - old);
+  const float A = k.adv, r = q.old.p ? expf(logp - k.old) : (logp == logp ? 1.f : logp);
   const float free = r * A, held = fminf(fmaxf(r, 1.f - q.clip_lo), 1.f + q.clip_hi) * A;
   // written so that a NaN ratio or advantage stays one (fminf and fmaxf drop it)
   float l = r != r ? r : -(free <= held ? free : held);
   float c = free <= held || r != r ? -free : 0.f;
   if (q.ref.p) {
-    const float d = q.ref.p[b * q.ref.sb + t * q.ref.st] - logp;
+    const float d = k.ref - logp;
     const float e = expm1f(d);  // e^d - 1 - d without losing a small d
     l += q.kl_coef * (e - d);
     c -= q.kl_coef * e;
@@ -170,13 +254,14 @@ __device__ __forceinline__ double cta_sum(double s) {
   return s;
 }
 
-// The CTA that is the last of `total` to come here sums x[0, n) into *out, times scale.
-__device__ __forceinline__ void last_one_sums(unsigned* ticket, unsigned total, const float* x, int64_t n, float scale,
-                                              float* out) {
+// CTAs come here with the part that they have done of `total`; the one that completes it sums x[0, n)
+// into *out, times scale.
+__device__ __forceinline__ void last_one_sums(unsigned* ticket, unsigned done, unsigned total, const float* x, int64_t n,
+                                              float scale, float* out) {
   __shared__ bool last;
   if (threadIdx.x == 0) {
     __threadfence();
-    last = atomicAdd(ticket, 1u) == total - 1;
+    last = atomicAdd(ticket, done) + done == total;
   }
   __syncthreads();
   if (!last) return;
@@ -188,138 +273,349 @@ __device__ __forceinline__ void last_one_sums(unsigned* ticket, unsigned total, 
 }
 
 // ---------------------------------------------------------------- rows
-struct MaxSum {
+struct alignas(8) MaxSum {  // written to other CTAs as one 8-byte vector
   float m, s;
 };
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, a.s + b.s};
-  return {m, a.s * exp_(a.m - m) + b.s * exp_(b.m - m)};
-}
 
-template <typename T>
-__device__ __forceinline__ void zero_row(const RowView<T>& out) {
-  Piece<T> z;
-#pragma unroll
-  for (int j = 0; j < Piece<T>::N; ++j) z.v[j] = from_f<T>(0.f);
-  for (int c = threadIdx.x; c < out.pieces; c += blockDim.x) out.store(out, c, z);
-}
-
-template <typename T>
-__device__ __forceinline__ void write_gradient(const RowView<T>& in, const RowView<T>& out, int64_t y, float m, float s,
-                                               float c) {
-  const float k = -c / s;
-  for (int i = threadIdx.x; i < in.pieces; i += blockDim.x) {
-    const Piece<T> x = in.load(i);
-    Piece<T> d;
-    const int64_t hit = y + in.off - (int64_t)i * Piece<T>::N;
-#pragma unroll
-    for (int j = 0; j < Piece<T>::N; ++j) {
-      float g = k * exp_(to_f(x.v[j]) - m);
-      if (hit == j) g += c;
-      d.v[j] = from_f<T>(g);
-    }
-    out.store(in, i, d);
+// The pieces of a CTA of a row's cluster: [lo, hi), in tiles of the shared memory's size.
+template <typename T, int THREADS>
+struct Slice {
+  static constexpr int kTile = kSliceBytes / 16;
+  int lo, hi;
+  __device__ Slice(const RowView<T>& v, int rank, int ctas) {
+    const int per = (v.pieces + ctas - 1) / ctas;
+    lo = min(rank * per, v.pieces);
+    hi = min(lo + per, v.pieces);
   }
+  __device__ __forceinline__ int tiles() const { return max(1, (hi - lo + kTile - 1) / kTile); }
+  __device__ __forceinline__ int begin(int tile) const { return lo + tile * kTile; }
+  __device__ __forceinline__ int end(int tile) const { return min(hi, lo + (tile + 1) * kTile); }
+  // Whether this thread is the one that has piece c.
+  __device__ __forceinline__ bool owns(int c) const { return c >= lo && c < hi && (c - lo) % kTile % THREADS == (int)threadIdx.x; }
+};
+
+// Brings a tile into shared memory: its whole pieces in one bulk copy, the row's ragged ends by their
+// threads. Complete after wait_tile.
+template <typename T, int THREADS>
+__device__ __forceinline__ void fill_tile(const RowView<T>& in, const Slice<T, THREADS>& s, int tile, uint4* buf, uint64_t* bar) {
+  const int b = s.begin(tile), e = s.end(tile);
+  const int wb = max(b, in.whole_lo), we = min(e, in.whole_hi);
+  if (threadIdx.x == 0) {
+    const uint32_t bytes = we > wb ? (uint32_t)(we - wb) * 16u : 0u;
+    const bool inside = LLMT_IN(in.at + wb * RowView<T>::N - in.off, in.at + max(we, wb) * RowView<T>::N - in.off, in.n, 601);
+    sm100::bar_arrive_expect_tx(bar, inside ? bytes : 0u);
+    if (bytes && inside) sm100::bulk_load(buf + (wb - b), in.p + (wb * RowView<T>::N - in.off), bytes, bar);
+  }
+  if (b < in.whole_lo && b < e && threadIdx.x == 0) buf[0] = load_part(in, b);
+  if (e > in.whole_hi && e - 1 >= b && e - 1 >= in.whole_lo && threadIdx.x == (unsigned)((e - 1 - b) % THREADS))
+    buf[e - 1 - b] = load_part(in, e - 1);
 }
 
-// One CTA per row: its maximum, sum and log-probability; with POLICY the loss and slope of its
-// token, with GRAD also the row of the gradient.
-template <typename T, bool POLICY, bool GRAD>
-__global__ void __launch_bounds__(kRowThreads) token_rows_kernel(TokenBatch a, PolicyArgs q, RowOut o) {
-  const int64_t n = blockIdx.x;
+// Pieces [b, e) of `like`, value(i) each, into the view `out` of the same row: whole pieces as such, the
+// row's ends, and everything where the two views lie differently, by elements.
+template <typename T, int THREADS, typename Value>
+__device__ __forceinline__ void store_pieces(const RowView<T>& out, const RowView<T>& like, int b, int e, Value value) {
+  if (out.off != like.off) {
+    for (int i = b + (int)threadIdx.x; i < e; i += THREADS) store_part(out, like, i, value(i));
+    return;
+  }
+  const int we = min(e, out.whole_hi);
+  uint4* const base = out.piece(0);
+  const bool inside = LLMT_IN(out.at + (int64_t)max(b, out.whole_lo) * Piece<T>::N - out.off,
+                              out.at + (int64_t)max(max(b, out.whole_lo), we) * Piece<T>::N - out.off, out.n, 603);
+  if (inside) {
+#pragma unroll 4
+    for (int i = b + (int)threadIdx.x; i < we; i += THREADS) {
+      const Piece<T> d = value(i);
+      if (i >= out.whole_lo) base[i] = make_uint4(d.u[0], d.u[1], d.u[2], d.u[3]);
+    }
+  }
+  if (b < out.whole_lo && b < e && threadIdx.x == 0) store_part(out, like, b, value(b));
+  if (e > out.whole_hi && e - 1 >= max(b, out.whole_lo) && threadIdx.x == (unsigned)((e - 1 - b) % THREADS))
+    store_part(out, like, e - 1, value(e - 1));
+}
+
+template <typename T, int THREADS>
+__device__ __forceinline__ void zero_row(const RowView<T>& out, int rank, int ctas) {
+  const Slice<T, THREADS> s(out, rank, ctas);
+  store_pieces<T, THREADS>(out, out, s.lo, s.hi, [](int) { return Piece<T>{{0u, 0u, 0u, 0u}}; });
+}
+
+// One tile of the gradient without the target's own term: k e^(z - M). For the 16-bit types the exponent
+// is one fused multiply-add, z log2(e) - M log2(e), off by 2^-24 of M log2(e); fp32 subtracts first.
+template <typename T>
+__device__ __forceinline__ float2 gradient_pair(float2 z, float m, float2 k2) {
+  const float2 l2 = make_float2(kLog2e, kLog2e);
+  float2 t;
+  if constexpr (sizeof(T) == 4) t = sm100::mul2(sm100::add2(z, make_float2(-m, -m)), l2);
+  else t = sm100::fma2(z, l2, make_float2(-m * kLog2e, -m * kLog2e));
+  return sm100::mul2(k2, make_float2(sm100::ex2_approx(t.x), sm100::ex2_approx(t.y)));
+}
+template <typename T>
+__device__ __forceinline__ Piece<T> gradient_piece(uint4 v, float m, float2 k2) {
+  const Piece<T> x = {{v.x, v.y, v.z, v.w}};
+  Piece<T> d;
+#pragma unroll
+  for (int h = 0; h < Piece<T>::N / 2; ++h) put_pair(d, h, gradient_pair<T>(pair_of(x, h), m, k2));
+  return d;
+}
+// The target's value once more, with its own term, by the thread that stored its piece.
+template <typename T>
+__device__ __forceinline__ void gradient_target(const RowView<T>& out, int y, float zy, float m, float k, float c) {
+  out.p[y] = from_f<T>(gradient_pair<T>(make_float2(zy, zy), m, make_float2(k, k)).x + c);
+}
+
+// Maximum and sum of the whole row from those of each warp, by one warp; a row with an infinite or NaN
+// maximum has sum NaN (its log-probability and gradient then are).
+__device__ __forceinline__ MaxSum join_warps(const MaxSum* part, int n) {
+  float m = -INFINITY, s = 0.f;
+  for (int i = threadIdx.x & 31; i < n; i += 32) m = max_nan(m, part[i].m);
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, w));
+  for (int i = threadIdx.x & 31; i < n; i += 32) s += part[i].s * exp_(part[i].m - m);
+  s = warp_sum(s);
+  if (!(fabsf(m) < INFINITY)) s = NAN;
+  return {m, s};
+}
+
+// The maximum's own term of a sum is exactly 1; the others are kShort short. The logarithm is in fp64:
+// one rounded to fp32 lies on the grid of the result (the difference of two 16-bit logits does too),
+// and what is added to it then only decides ties, always to one side.
+__device__ __forceinline__ float row_logp(float zy, MaxSum r) {
+  const double s = (double)r.s;
+  return (float)((double)(zy - r.m) - (log(s) + kShort * (double)(1.f - 1.f / r.s)));
+}
+
+__device__ int g_error = 0;  // 1: a copy did not arrive within its wait's limit (the results are void)
+
+// All threads wait for a tile. One warp polls while the others rest at the CTA's barrier: sixteen polling
+// warps took more of the SM's issue slots than the row's arithmetic (21.5 instructions a value against 9.5).
+// After a wait that ran out, one more for the copy: the CTA must not end under it.
+__device__ __forceinline__ void wait_tile(uint64_t* bar, uint32_t parity) {
+  if (threadIdx.x < 32 && !sm100::wait_bar(bar, parity, &g_error, 1)) sm100::wait_bar(bar, parity, &g_error, 1);
+  __syncthreads();
+  sm100::bar_try_wait(bar, parity);  // done: each thread sees the copy for itself
+}
+
+// One cluster per row: its maximum, sum and log-probability; with POLICY the loss and slope of its
+// token, with GRAD also the row of the gradient. The row lies in shared memory from its one read to its
+// gradient; the CTAs on a SM work on different rows, so that one's copy runs under another's arithmetic.
+template <typename T, int THREADS, bool POLICY, bool GRAD>
+__global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(TokenBatch a, PolicyArgs q, RowOut o, int ctas) {
+  constexpr int kWarps = THREADS / 32;
+  extern __shared__ uint4 buf[];
+  __shared__ MaxSum part[kMaxCluster * kWarps];
+  __shared__ float s_row[3];
+  __shared__ uint64_t bar;
+  const int64_t n = blockIdx.x / ctas;
+  const int rank = (int)(blockIdx.x % ctas), warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
   const int b = (int)(n / a.T), t = (int)(n % a.T);
   int64_t y;
-  const bool counts = token_counts(a, b, t, &y);
-  const RowView<T> in((T*)a.z + b * a.zsb + t * a.zst, a.V);
-  const RowView<T> out(GRAD ? (T*)o.dz + b * o.sb + t * o.st : (T*)a.z, a.V);
-  if (n == 0 && !POLICY && threadIdx.x == 0 && o.ticket) *o.ticket = 0;
+  const bool counts = token_counts(a, b, t, &y);  // the same for the whole cluster
+  const RowView<T> in((T*)a.z, b * a.zsb + t * a.zst, a.zn, a.V);
+  const RowView<T> out(GRAD ? (T*)o.dz : (T*)a.z, GRAD ? b * o.sb + t * o.st : 0, GRAD ? o.dn : a.zn, a.V);
+  pdl_trigger();
   if (!counts) {
-    if (threadIdx.x == 0) {
+    pdl_wait();
+    if (rank == 0 && threadIdx.x == 0) {
+      if (n == 0 && !POLICY && o.ticket) *o.ticket = 0;
       o.logp[n] = 0.f;
       if (o.stats) o.stats[n] = make_float2(0.f, 1.f);
       if (POLICY) o.loss_rows[n] = 0.f, o.coef[n] = 0.f;
     }
-    if (GRAD) zero_row(out);
+    if (GRAD) zero_row<T, THREADS>(out, rank, ctas);
   } else {
-    const float zy = to_f(in.p[y]);
-    MaxSum ms = {-INFINITY, 0.f};
-    for (int i = threadIdx.x; i < in.pieces; i += blockDim.x) {
-      const Piece<T> x = in.load(i);
-      float f[Piece<T>::N], top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < Piece<T>::N; ++j) {
-        f[j] = to_f(x.v[j]);
-        top = fmaxf(top, f[j]);
-      }
-      const float at = top == -INFINITY ? 0.f : top;
-#pragma unroll
-      for (int j = 0; j < Piece<T>::N; ++j) sum += exp_(f[j] - at);
-      ms = join(ms, {top, sum});
-    }
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1)
-      ms = join(ms, {__shfl_xor_sync(0xffffffffu, ms.m, w), __shfl_xor_sync(0xffffffffu, ms.s, w)});
-    __shared__ MaxSum part[kRowThreads / 32];
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = ms;
-    __syncthreads();
-    ms = part[0];
-    for (int i = 1; i < (int)(blockDim.x >> 5); ++i) ms = join(ms, part[i]);
-    const float logp = (zy - ms.m) - logf(ms.s);
-    float loss = 0.f, slope = 0.f;
-    if (POLICY) policy_token(q, b, t, logp, token_weight(o.count, a.B, b, q.reduction), &loss, &slope);
+    const Slice<T, THREADS> s(in, rank, ctas);
+    const int tiles = s.tiles();
     if (threadIdx.x == 0) {
-      o.logp[n] = logp;
-      if (o.stats) o.stats[n] = make_float2(ms.m, ms.s);
-      if (POLICY) o.loss_rows[n] = loss, o.coef[n] = slope;
+      sm100::bar_init(&bar, 1);
+      sm100::fence_barrier_init();
+      sm100::fence_proxy_async_smem();
+    }
+    fill_tile(in, s, 0, buf, &bar);  // thread 0 made the barrier
+    // (a CTA's shared memory may be written by others once it has begun)
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    // what the token's loss needs, while the row is on its way
+    const float zy = to_f(in.p[y]);
+    PolicyToken token = {};
+    float weight = 0.f;
+    if (POLICY && warp == 0) {
+      token = load_token(q, b, t);
+      pdl_wait();  // the counts
+      weight = token_weight(o.count, a.B, b, q.reduction);
+    }
+    uint32_t parity = 0;
+    MaxSum ms = {-INFINITY, 0.f};
+    for (int tile = 0; tile < tiles; ++tile) {
+      if (tile > 0) {
+        __syncthreads();  // the tile before has been read
+        if (threadIdx.x == 0) sm100::fence_proxy_async_smem();
+        fill_tile(in, s, tile, buf, &bar);
+      }
+      wait_tile(&bar, parity);
+      parity ^= 1;
+      const int count = s.end(tile) - s.begin(tile);
+      float m = ms.m;
+#pragma unroll 4
+      for (int i = threadIdx.x; i < count; i += THREADS) {
+        const uint4 v = buf[i];
+        m = piece_max(Piece<T>{{v.x, v.y, v.z, v.w}}, m);
+      }
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, w));
+      const float at = m == -INFINITY ? 0.f : m;
+      float2 sum = make_float2(ms.s == 0.f ? 0.f : ms.s * exp_(ms.m - at), 0.f);
+#pragma unroll 4
+      for (int i = threadIdx.x; i < count; i += THREADS) {
+        const uint4 v = buf[i];
+        const Piece<T> x = {{v.x, v.y, v.z, v.w}};
+#pragma unroll
+        for (int h = 0; h < Piece<T>::N / 2; ++h) sum = add_exp(pair_of(x, h), make_float2(-at, -at), sum);
+      }
+      ms.m = m;
+      ms.s = sum.x + sum.y;
+    }
+    ms.s = warp_sum(ms.s);
+    // every warp's pair to every CTA of the cluster
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (lane < ctas) {
+      MaxSum* slot = &part[rank * kWarps + warp];
+      if (ctas == 1) {
+        *slot = ms;
+      } else {
+        const uint32_t to = sm100::cluster_map(slot, lane);
+        asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(ms.m), "f"(ms.s) : "memory");
+      }
+    }
+    if (ctas == 1) __syncthreads();
+    else sm100::cluster_sync();
+    pdl_wait();  // nothing is written before
+    if (warp == 0) {
+      ms = join_warps(part, ctas * kWarps);
+      const float logp = row_logp(zy, ms);
+      float loss = 0.f, slope = 0.f;
+      if (POLICY) policy_token(q, token, logp, weight, &loss, &slope);
+      if (lane == 0) {
+        if (rank == 0) {
+          if (n == 0 && !POLICY && o.ticket) *o.ticket = 0;
+          o.logp[n] = logp;
+          if (o.stats) o.stats[n] = make_float2(ms.m, ms.s);
+          if (POLICY) o.loss_rows[n] = loss, o.coef[n] = slope;
+        }
+        s_row[0] = ms.m;
+        s_row[1] = -slope / ms.s;
+        s_row[2] = slope;
+      }
     }
     if (GRAD) {
-      if (slope == 0.f) zero_row(out);
-      else write_gradient(in, out, y, ms.m, ms.s, slope * (o.grad_out ? *o.grad_out : 1.f));
+      __syncthreads();
+      const float m = s_row[0], k = s_row[1], c = s_row[2];
+      if (c == 0.f) {
+        zero_row<T, THREADS>(out, rank, ctas);
+      } else {
+        for (int tile = tiles - 1; tile >= 0; --tile) {  // the last one is still there
+          if (tile != tiles - 1) {
+            __syncthreads();
+            if (threadIdx.x == 0) sm100::fence_proxy_async_smem();
+            fill_tile(in, s, tile, buf, &bar);
+            wait_tile(&bar, parity);
+            parity ^= 1;
+          }
+          const int first = s.begin(tile);
+          store_pieces<T, THREADS>(out, in, first, s.end(tile),
+                                   [&](int i) { return gradient_piece<T>(buf[i - first], m, make_float2(k, k)); });
+        }
+        if (s.owns(((int)y + in.off) / Piece<T>::N)) gradient_target(out, (int)y, zy, m, k, c);
+      }
     }
   }
-  if (POLICY) last_one_sums(o.ticket, gridDim.x, o.loss_rows, gridDim.x, 1.f, o.loss);
+}
+
+// The loss from its rows, in a fixed order. A kernel of its own: a ticket taken by each row's CTA needs a
+// fence after the row's loss, and the fence waits for the CTA's gradient to reach memory (18 us of 120
+// at 4096 rows of 32000 bf16).
+__global__ void __launch_bounds__(1024) sum_rows_kernel(const float* x, int64_t n, float* out) {
+  pdl_wait();
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) s += (double)x[i];
+  s = cta_sum(s);
+  if (threadIdx.x == 0) *out = (float)s;
 }
 
 // Gradient rows from the saved maxima and sums and the slope of each token. With skip_one the
 // buffer already holds the gradient for an incoming gradient of 1.
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) grad_rows_kernel(TokenBatch a, RowOut o, bool skip_one) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 768 / THREADS) grad_rows_kernel(TokenBatch a, RowOut o, bool skip_one, int ctas) {
+  extern __shared__ uint4 buf[];
+  __shared__ uint64_t bar;
+  pdl_trigger();
   const float g = o.grad_out ? *o.grad_out : 1.f;
   if (skip_one && g == 1.f) return;
   // the last rows first: the pass before this one left them in L2
-  const int64_t n = gridDim.x - 1 - (int64_t)blockIdx.x;
+  const int64_t n = (gridDim.x - 1 - (int64_t)blockIdx.x) / ctas;
+  const int rank = (int)((gridDim.x - 1 - blockIdx.x) % ctas);
   const int b = (int)(n / a.T), t = (int)(n % a.T);
-  const RowView<T> in((T*)a.z + b * a.zsb + t * a.zst, a.V);
-  const RowView<T> out((T*)o.dz + b * o.sb + t * o.st, a.V);
-  const float c = o.coef[n];
-  if (c == 0.f) {
-    zero_row(out);
+  int64_t y;
+  const bool counts = token_counts(a, b, t, &y);
+  const RowView<T> in((T*)a.z, b * a.zsb + t * a.zst, a.zn, a.V);
+  const RowView<T> out((T*)o.dz, b * o.sb + t * o.st, o.dn, a.V);
+  const Slice<T, THREADS> s(in, rank, ctas);
+  const int tiles = s.tiles();
+  const bool mine = counts && s.owns(((int)y + in.off) / Piece<T>::N);
+  const float zy = mine ? to_f(in.p[y]) : 0.f;
+  if (threadIdx.x == 0) {
+    sm100::bar_init(&bar, 1);
+    sm100::fence_barrier_init();
+    sm100::fence_proxy_async_smem();
+  }
+  // the copy runs while the slopes are waited for, unless the token has none
+  if (counts) fill_tile(in, s, tiles - 1, buf, &bar);
+  pdl_wait();
+  const float c = o.coef[n] * g;
+  if (counts) wait_tile(&bar, 0);
+  if (!counts || c == 0.f) {
+    zero_row<T, THREADS>(out, rank, ctas);
     return;
   }
   const float2 ms = o.stats[n];
-  write_gradient(in, out, a.tgt.p[b * a.tgt.sb + t * a.tgt.st], ms.x, ms.y, c * g);
+  const float k = -c / ms.y;
+  uint32_t parity = 1;
+  for (int tile = tiles - 1; tile >= 0; --tile) {
+    const int first = s.begin(tile);
+    if (tile != tiles - 1) {
+      __syncthreads();
+      if (threadIdx.x == 0) sm100::fence_proxy_async_smem();
+      fill_tile(in, s, tile, buf, &bar);
+      wait_tile(&bar, parity);
+      parity ^= 1;
+    }
+    store_pieces<T, THREADS>(out, in, first, s.end(tile),
+                             [&](int i) { return gradient_piece<T>(buf[i - first], ms.x, make_float2(k, k)); });
+  }
+  if (mine) gradient_target(out, (int)y, zy, ms.x, k, c);
 }
 
 // ---------------------------------------------------------------- losses on log-probabilities
 __global__ void __launch_bounds__(kPairThreads) policy_tokens_kernel(TokenBatch a, PolicyArgs q, const float* logp, RowOut o) {
   const int b = blockIdx.x;
-  const float w = token_weight(o.count, a.B, b, q.reduction);
+  const float w = token_weight(o.count, a.B, b, q.reduction);  // each warp for itself
   for (int t = threadIdx.x; t < a.T; t += blockDim.x) {
     const int64_t n = (int64_t)b * a.T + t;
     int64_t y;
     float loss = 0.f, slope = 0.f;
-    if (token_counts(a, b, t, &y)) policy_token(q, b, t, logp[n], w, &loss, &slope);
+    if (token_counts(a, b, t, &y)) policy_token(q, load_token(q, b, t), logp[n], w, &loss, &slope);
     o.loss_rows[n] = loss;
     o.coef[n] = slope;
   }
   __syncthreads();
-  last_one_sums(o.ticket, gridDim.x, o.loss_rows, (int64_t)a.B * a.T, 1.f, o.loss);
+  last_one_sums(o.ticket, 1, gridDim.x, o.loss_rows, (int64_t)a.B * a.T, 1.f, o.loss);
 }
 
 // One CTA per pair.
 __global__ void __launch_bounds__(kPairThreads) preference_kernel(TokenBatch a, PreferenceArgs q, const float* logp, RowOut o) {
   const int p = blockIdx.x, P = gridDim.x;
+  pdl_trigger();
+  pdl_wait();  // the log-probabilities
   double gain[2];
   int number[2];
 #pragma unroll 1
@@ -362,18 +658,71 @@ __global__ void __launch_bounds__(kPairThreads) preference_kernel(TokenBatch a, 
     if (threadIdx.x == 0) o.rewards[b] = (float)((double)q.beta * gain[side]);
   }
   if (threadIdx.x == 0) o.loss_rows[p] = loss;
-  last_one_sums(o.ticket, P, o.loss_rows, P, 1.f / (float)P, o.loss);
+  last_one_sums(o.ticket, 1, P, o.loss_rows, P, 1.f / (float)P, o.loss);
 }
 
+// CTAs and threads for a row: as many CTAs as hold it (64 KB each), and more while the rows would leave
+// SMs without work; fewer threads for short rows.
+struct RowShape {
+  int ctas, threads, bytes;
+};
+RowShape row_shape(const TokenBatch& a) {
+  const int e = a.dtype == 2 ? 4 : 2;
+  const int64_t pieces = cdiv((int64_t)a.V * e, 16) + 1, n = (int64_t)a.B * a.T;
+  RowShape r{1, kMaxThreads, 0};
+  while (r.ctas < kMaxCluster && pieces * 16 > (int64_t)r.ctas * kSliceBytes) r.ctas *= 2;
+  while (r.ctas < kMaxCluster && n * r.ctas * 2 <= 4 * sm_count() && pieces >= 512 * r.ctas) r.ctas *= 2;
+  const int64_t per = cdiv(pieces, (int64_t)r.ctas);
+  r.threads = per <= 512 ? 128 : 256;
+  r.bytes = (int)std::min<int64_t>(per * 16, kSliceBytes);
+  return r;
+}
+
+// pdl: may start while the kernel before it in the stream, one of this file, runs.
+template <typename... K, typename... A>
+cudaError_t launch_rows(void (*kernel)(K...), const TokenBatch& a, RowShape r, int smem, bool pdl, cudaStream_t st, A&&... args) {
+  const int64_t n = (int64_t)a.B * a.T;
+  LLMT_REQUIRE(n * r.ctas <= 0x7fffffff, "loss rows: too many tokens");
+  if (smem > 48 * 1024)
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceBytes)) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = (unsigned)(n * r.ctas);
+  cfg.blockDim = r.threads;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)r.ctas, 1, 1};
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = r.ctas > 1 ? attr : attr + 1;
+  cfg.numAttrs = (r.ctas > 1 ? 1 : 0) + (pdl ? 1 : 0);
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(args)...);
+}
+
+template <typename T, bool POLICY, bool GRAD>
+cudaError_t rows_of(const TokenBatch& a, RowShape r, const PolicyArgs& q, const RowOut& o, cudaStream_t st) {
+  switch (r.threads) {
+    case 128: return launch_rows(token_rows_kernel<T, 128, POLICY, GRAD>, a, r, r.bytes, POLICY, st, a, q, o, r.ctas);
+    default: return launch_rows(token_rows_kernel<T, 256, POLICY, GRAD>, a, r, r.bytes, POLICY, st, a, q, o, r.ctas);
+  }
+}
 template <bool POLICY, bool GRAD>
 cudaError_t rows(const TokenBatch& a, const PolicyArgs& q, const RowOut& o, cudaStream_t st) {
-  const unsigned n = (unsigned)((int64_t)a.B * a.T);
+  const RowShape r = row_shape(a);
   switch (a.dtype) {
-    case 0: token_rows_kernel<bf16, POLICY, GRAD><<<n, kRowThreads, 0, st>>>(a, q, o); break;
-    case 1: token_rows_kernel<__half, POLICY, GRAD><<<n, kRowThreads, 0, st>>>(a, q, o); break;
-    default: token_rows_kernel<float, POLICY, GRAD><<<n, kRowThreads, 0, st>>>(a, q, o); break;
+    case 0: return rows_of<bf16, POLICY, GRAD>(a, r, q, o, st);
+    case 1: return rows_of<__half, POLICY, GRAD>(a, r, q, o, st);
+    default: return rows_of<float, POLICY, GRAD>(a, r, q, o, st);
   }
-  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t grad_rows_of(const TokenBatch& a, const RowOut& o, bool skip_one, bool pdl, cudaStream_t st) {
+  const RowShape r = row_shape(a);
+  switch (r.threads) {
+    case 128: return launch_rows(grad_rows_kernel<T, 128>, a, r, r.bytes, pdl, st, a, o, skip_one, r.ctas);
+    default: return launch_rows(grad_rows_kernel<T, 256>, a, r, r.bytes, pdl, st, a, o, skip_one, r.ctas);
+  }
 }
 
 cudaError_t check(const TokenBatch& a) {
@@ -393,7 +742,8 @@ cudaError_t policy_rows(const TokenBatch& a, const PolicyArgs& q, const RowOut& 
   if (cudaError_t e = check(a)) return e;
   count_tokens_kernel<<<a.B, 256, 0, st>>>(a, o.count, o.ticket);
   if (cudaError_t e = cudaGetLastError()) return e;
-  return o.dz ? rows<true, true>(a, q, o, st) : rows<true, false>(a, q, o, st);
+  if (cudaError_t e = o.dz ? rows<true, true>(a, q, o, st) : rows<true, false>(a, q, o, st)) return e;
+  return launch_pdl_if(true, sum_rows_kernel, 1, 1024, 0, st, (const float*)o.loss_rows, (int64_t)a.B * a.T, o.loss);
 }
 
 cudaError_t policy_tokens(const TokenBatch& a, const PolicyArgs& q, const float* logp, const RowOut& o, cudaStream_t st) {
@@ -410,19 +760,26 @@ cudaError_t preference_tokens(const TokenBatch& a, const PreferenceArgs& q, cons
   LLMT_REQUIRE(a.B % 2 == 0, "preference loss: the batch holds the chosen sequences, then as many rejected ones");
   if (!ticket_ready)
     if (cudaError_t e = cudaMemsetAsync(o.ticket, 0, sizeof(unsigned), st)) return e;
-  preference_kernel<<<a.B / 2, kPairThreads, 0, st>>>(a, q, logp, o);
-  return cudaGetLastError();
+  return launch_pdl_if(ticket_ready, preference_kernel, a.B / 2, kPairThreads, 0, st, a, q, logp, o);
 }
 
-cudaError_t grad_rows(const TokenBatch& a, const RowOut& o, bool skip_one, cudaStream_t st) {
+cudaError_t grad_rows(const TokenBatch& a, const RowOut& o, bool skip_one, bool after_loss, cudaStream_t st) {
   if (cudaError_t e = check(a)) return e;
-  const unsigned n = (unsigned)((int64_t)a.B * a.T);
   switch (a.dtype) {
-    case 0: grad_rows_kernel<bf16><<<n, kRowThreads, 0, st>>>(a, o, skip_one); break;
-    case 1: grad_rows_kernel<__half><<<n, kRowThreads, 0, st>>>(a, o, skip_one); break;
-    default: grad_rows_kernel<float><<<n, kRowThreads, 0, st>>>(a, o, skip_one); break;
+    case 0: return grad_rows_of<bf16>(a, o, skip_one, after_loss, st);
+    case 1: return grad_rows_of<__half>(a, o, skip_one, after_loss, st);
+    default: return grad_rows_of<float>(a, o, skip_one, after_loss, st);
   }
-  return cudaGetLastError();
+}
+
+int loss_error_code(bool reset) {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, g_error, sizeof(int));
+  if (reset) {
+    const int z = 0;
+    cudaMemcpyToSymbol(g_error, &z, sizeof(int));
+  }
+  return v;
 }
 
 }  // namespace llmt

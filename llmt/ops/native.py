@@ -18,7 +18,7 @@ EPI_BF16, EPI_F32, EPI_SWIGLU, EPI_SWIGLU_BWD, EPI_ROPE, EPI_CE_FWD, EPI_CE_BWD 
 
 
 # Kernels launched per call of an extension entry point (1 unless listed).
-_KERNELS_PER_CALL = {"flash_attn_bwd": 3, "gemm_error_code": 0, "attn_error_code": 0, "dp_error_code": 0,
+_KERNELS_PER_CALL = {"flash_attn_bwd": 3, "gemm_error_code": 0, "attn_error_code": 0, "loss_error_code": 0, "dp_error_code": 0,
                      "set_reserved_sms": 0, "reserved_sms": 0,
                      "ipc_alloc": 0, "ipc_open": 0, "ipc_close": 0, "ipc_free": 0, "tensor_from_ptr": 0,
                      "sm_count": 0, "MultiPlan": 0, "bounds_error": 0, "bounds_checking": 0, "fp8_quant": 2, "fp8_amax_slots": 0, "mx_sf_bytes": 0, "gemm_plan": 0}
@@ -455,3 +455,8 @@ def flash_attn_bwd(do, qkv, o, lse, cos, sin, B, T, H, KV, hd, causal=True, scal
 
 def attn_error_code(reset=False) -> int:
     return ext().attn_error_code(reset)
+
+
+def loss_error_code(reset=False) -> int:
+    """Sticky code of the first bounded-wait timeout a kernel of the losses over rows hit (0 = none)."""
+    return ext().loss_error_code(reset)

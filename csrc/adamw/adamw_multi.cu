@@ -49,32 +49,39 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t top, int places, uint32_
 __device__ __forceinline__ uint32_t scale_byte_m(uint32_t top) { return scale_byte(top, 8, 0x600000u); }   // 448
 __device__ __forceinline__ uint32_t scale_byte_v(uint32_t top) { return scale_byte(top, 33, 0x700000u); }  // 1.875 2^33
 
-// Both codes are the top bits of an fp32 number: scaled so that the format's subnormals are fp32's
+// Both codes are bits 20 to 27 of an fp32 number: scaled so that the format's subnormals are fp32's
 // subnormals, adding 20 random bits below the kept ones and cutting rounds up with the right
-// probability, in the normal and the subnormal range alike.
-__device__ __forceinline__ uint32_t encode_m(float m, uint32_t e, uint32_t noise) {
-  if (m != m) return 0x7fu;
-  const float y = __fmul_rn(__fmul_rn(fabsf(m), pow2_of(254u - e)), 0x1p-120f);
-  return min((__float_as_uint(y) + noise) >> 20, 126u) | (m < 0.f ? 0x80u : 0u);
+// probability, in the normal and the subnormal range alike. Here they are shifted to the top byte, where
+// four of them are gathered by byte permutations, as the noise is made: the kernel is bound by its
+// integer instructions. noise: bits 8 to 23 random, bit 7 set (half a last step). A block's scale keeps
+// every finite value within the format; infinities and NaN are put right afterwards (code_of_bad_*).
+__device__ __forceinline__ uint32_t encode_m(float m, float unscale, uint32_t noise) {  // without the sign
+  return (__float_as_uint(__fmul_rn(__fmul_rn(fabsf(m), unscale), 0x1p-120f)) << 4) + noise;
 }
-__device__ __forceinline__ uint32_t encode_v(float v, uint32_t e, uint32_t noise) {
-  const float y = __fmul_rn(__fmul_rn(v, pow2_of(254u - e)), 0x1p-129f);
-  const uint32_t c = min((__float_as_uint(y) + noise) >> 20, 255u);
-  return v > 0.f ? max(c, 1u) : c;
+__device__ __forceinline__ uint32_t encode_v(float v, float unscale, uint32_t noise) {
+  const uint32_t y = (__float_as_uint(__fmul_rn(__fmul_rn(v, unscale), 0x1p-129f)) << 4) + noise;
+  return max(y, min(__float_as_uint(v), 1u) << 24);  // v >= 0: a non-zero one keeps a non-zero code
 }
-__device__ __forceinline__ float decode_m(uint32_t code, float scale) {
-  const float y = __uint_as_float((code & 0x7fu) << 20) * 0x1p120f;
-  const float x = (code & 0x7fu) == 0x7fu ? NAN : y * scale;
-  return code & 0x80u ? -x : x;
+__device__ __forceinline__ uint32_t code_of_bad_m(float m, uint32_t code) { return m != m ? 0x7fu : fabsf(m) == INFINITY ? 126u : code; }
+__device__ __forceinline__ uint32_t code_of_bad_v(float v, uint32_t code) { return v <= 3.4028235e38f ? code : 255u; }
+__device__ __forceinline__ uint32_t sign_m(float m) { return (__float_as_uint(m) >> 24) & 0x80u; }
+
+__device__ __forceinline__ float2 decode_m2(uint32_t codes, float scale) {  // two codes in the low 16 bits
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);  // exact
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return make_float2(f.x * scale, f.y * scale);
 }
-__device__ __forceinline__ float decode_v(uint32_t code, float scale) {
-  return __uint_as_float(code << 20) * 0x1p64f * 0x1p65f * scale;
+__device__ __forceinline__ float decode_m(uint32_t code, float scale) { return decode_m2(code & 0xffu, scale).x; }
+// scale_2_29: 2^29 times the block's scale (codes are units of 2^-129 as fp32 bits; two exact steps).
+__device__ __forceinline__ float decode_v(uint32_t code, float scale_2_29) {
+  return __uint_as_float(code << 20) * 0x1p100f * scale_2_29;
 }
 
 // 32 mixed bits of place i: two rounds of multiplication and xor-shift; the odd constants are
 // digits of e, of the square root of two and of the golden ratio.
-__device__ __forceinline__ uint32_t place_hash(int64_t i, uint32_t seed) {
-  uint32_t x = ((uint32_t)i ^ ((uint32_t)(i >> 32) * 0x6A09E667u)) * 0x9E3779B1u + seed;
+__device__ __forceinline__ uint32_t high_mix(int64_t i) { return (uint32_t)(i >> 32) * 0x6A09E667u; }
+__device__ __forceinline__ uint32_t place_hash(uint32_t low, uint32_t high, uint32_t seed) {
+  uint32_t x = (low ^ high) * 0x9E3779B1u + seed;
   x = (x ^ (x >> 16)) * 0xB7E15163u;
   x = (x ^ (x >> 15)) * 0x6A09E667u;
   return x ^ (x >> 16);
@@ -85,11 +92,14 @@ struct StepConst {
   uint32_t seed;
 };
 
+// The quotient by the approximate square root and reciprocal (2^-22 of the update); the moments as written.
 __device__ __forceinline__ void update(const StepConst& k, float decay, float g, float& p, float& m, float& v) {
   g = __fmul_rn(g, k.grad_scale);
   m = __fadd_rn(__fmul_rn(m, k.b1), __fmul_rn(g, k.c1));
   v = __fadd_rn(__fmul_rn(v, k.b2), __fmul_rn(__fmul_rn(g, k.c2), g));
-  p = p * decay - k.step_size * (m / (sqrtf(v) * k.root + k.eps));
+  float root;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v));
+  p = p * decay - k.step_size * __fdividef(m, root * k.root + k.eps);
 }
 
 __device__ __forceinline__ StepConst step_const(const MultiHyper& h) {
@@ -108,80 +118,240 @@ __device__ __forceinline__ StepConst step_const(const MultiHyper& h) {
   return k;
 }
 
-template <typename G, int BITS, int CAP>
-__global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_constant__ Batch<CAP> batch, MultiHyper h,
-                                                               MultiState s, int64_t blocks, bool last_launch) {
-  const StepConst k = step_const(h);
-  const int lane = threadIdx.x & 31;
-  const int64_t stride = (int64_t)gridDim.x * (kThreads / 32);
-  for (int64_t w = blockIdx.x * (int64_t)(kThreads / 32) + (threadIdx.x >> 5); w < blocks; w += stride) {
-    int lo = 0, hi = batch.count - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (batch.t[mid].first_work <= w) lo = mid;
-      else hi = mid - 1;
-    }
-    const MultiTensor& t = batch.t[lo];
-    const int64_t in_t = w - t.first_work, at = in_t * kBlock;
-    const int64_t blk = t.first_block + in_t;  // in the state buffers
-    const int n = (int)min((int64_t)kBlock, t.n - at);
-    const float decay = 1.f - k.lr * t.wd;
-    float m[8], v[8];
-    float sm = 1.f, sv = 1.f;
-    if (BITS == 8) {
-      sm = pow2_of(s.ms[blk]);
-      sv = pow2_of(s.vs[blk]);
-    }
-    uint32_t top_m = 0, top_v = 0;
+// 32 bytes at once (the widest load and store of sm_100): a lane's eight fp32 values.
+__device__ __forceinline__ void ld8(const float* p, float (&x)[8]) {
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void st8(float* p, const float (&x)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]),
+               "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
+               : "memory");
+}
+
+// Exponent bytes of a block (the whole warp calls it).
+struct Scales {
+  uint32_t m, v;
+};
+__device__ __forceinline__ Scales block_scales(float top_m, float top_v) {
+  return {scale_byte_m(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m))),
+          scale_byte_v(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)))};
+}
+// The random bits of each moment from a place's 32: the upper 16 and the lower 16.
+__device__ __forceinline__ uint32_t noise_m(uint32_t r) { return __byte_perm(r, 0x80u, 0x5324); }
+__device__ __forceinline__ uint32_t noise_v(uint32_t r) { return __byte_perm(r, 0x80u, 0x5104); }
+// The top bytes of four words.
+__device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+
+// A whole block of a tensor on 32-byte borders (16 for 16-bit gradients and copies): all its loads are
+// issued before anything is computed.
+template <typename G, int BITS>
+__device__ __forceinline__ void whole_block(const MultiTensor& t, const MultiHyper& h, const MultiState& s, const StepConst& k,
+                                            int64_t at, int64_t blk, int lane) {
+  const float decay = 1.f - k.lr * t.wd;
+  const int64_t i = at + 8 * lane, si = blk * kBlock + 8 * lane;
+  float p[8], g[8], m[8], v[8];
+  uint4 g16;
+  if constexpr (sizeof(G) == 4) ld8(static_cast<const float*>(t.g) + i, g);
+  else g16 = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(t.g) + i);
+  ld8(t.p + i, p);
+  uint2 mc, vc;
+  uint32_t em = 0, ev = 0;
+  if constexpr (BITS == 8) {
+    mc = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.m) + si);
+    vc = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(s.v) + si);
+    em = s.ms[blk];
+    ev = s.vs[blk];
+  } else {
+    ld8(static_cast<const float*>(s.m) + si, m);
+    ld8(static_cast<const float*>(s.v) + si, v);
+  }
+  if constexpr (sizeof(G) == 2) {
+    const uint32_t u[4] = {g16.x, g16.y, g16.z, g16.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int i = lane + 32 * j;
-      m[j] = v[j] = 0.f;
-      if (i >= n) continue;
-      const int64_t si = blk * kBlock + i;
-      float p = t.p[at + i];
-      float g;
-      if constexpr (sizeof(G) == 4) g = static_cast<const float*>(t.g)[at + i];
-      else g = __bfloat162float(static_cast<const bf16*>(t.g)[at + i]);
-      if (BITS == 8) {
-        m[j] = decode_m(static_cast<const uint8_t*>(s.m)[si], sm);
-        v[j] = decode_v(static_cast<const uint8_t*>(s.v)[si], sv);
-      } else {
-        m[j] = static_cast<const float*>(s.m)[si];
-        v[j] = static_cast<const float*>(s.v)[si];
-      }
-      update(k, decay, g, p, m[j], v[j]);
-      t.p[at + i] = p;
-      if (t.p16) static_cast<bf16*>(t.p16)[at + i] = __float2bfloat16_rn(p);
-      if (h.zero_grad) {
-        if constexpr (sizeof(G) == 4) static_cast<float*>(t.g)[at + i] = 0.f;
-        else static_cast<bf16*>(t.g)[at + i] = __float2bfloat16_rn(0.f);
-      }
-      if (BITS == 32) {
-        static_cast<float*>(s.m)[si] = m[j];
-        static_cast<float*>(s.v)[si] = v[j];
-      }
-      // (a NaN does not set the scale)
-      if (fabsf(m[j]) <= INFINITY) top_m = max(top_m, __float_as_uint(fabsf(m[j])));
-      if (v[j] <= INFINITY) top_v = max(top_v, __float_as_uint(v[j]));
+    for (int j = 0; j < 4; ++j) {
+      g[2 * j] = __uint_as_float(u[j] << 16);
+      g[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
     }
-    if (BITS == 8) {
-      const uint32_t em = scale_byte_m(__reduce_max_sync(0xffffffffu, top_m));
-      const uint32_t ev = scale_byte_v(__reduce_max_sync(0xffffffffu, top_v));
+  }
+  if constexpr (BITS == 8) {
+    const float sm = pow2_of(em), sv = pow2_of(ev + 29u);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = decode_m2((j < 2 ? mc.x : mc.y) >> (16 * (j & 1)), sm);
+      m[2 * j] = f.x;
+      m[2 * j + 1] = f.y;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = decode_v(((j < 4 ? vc.x : vc.y) >> (8 * (j & 3))) & 0xffu, sv);
+  }
+  float top_m = 0.f, top_v = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    update(k, decay, g[j], p[j], m[j], v[j]);
+    top_m = fmaxf(top_m, fabsf(m[j]));  // (a NaN does not set the scale)
+    top_v = fmaxf(top_v, v[j]);
+  }
+  st8(t.p + i, p);
+  if (t.p16) {
+    BF16x8 o = float_to_bf16x8(p);
+    *reinterpret_cast<BF16x8*>(static_cast<bf16*>(t.p16) + i) = o;
+  }
+  if (h.zero_grad) {
+    const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if constexpr (sizeof(G) == 4) st8(static_cast<float*>(t.g) + i, z);
+    else *reinterpret_cast<uint4*>(static_cast<bf16*>(t.g) + i) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  if constexpr (BITS == 8) {
+    const Scales e = block_scales(top_m, top_v);
+    const float um = pow2_of(254u - e.m), uv = pow2_of(254u - e.v);
+    const uint32_t high = high_mix(si), low = (uint32_t)si;  // one high word for the block
+    uint32_t cm[2], cv[2];
+    float bad = 0.f;  // becomes NaN where a moment is infinite or NaN
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint32_t a[4], b[4], sg[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t r = place_hash(low + 4 * q + j, high, k.seed);
+        a[j] = encode_m(m[4 * q + j], um, noise_m(r));
+        b[j] = encode_v(v[4 * q + j], uv, noise_v(r));
+        sg[j] = __float_as_uint(m[4 * q + j]);
+        bad = fmaf(m[4 * q + j], 0.f, fmaf(v[4 * q + j], 0.f, bad));
+      }
+      cm[q] = top_bytes(a[0], a[1], a[2], a[3]) | (top_bytes(sg[0], sg[1], sg[2], sg[3]) & 0x80808080u);
+      cv[q] = top_bytes(b[0], b[1], b[2], b[3]);
+    }
+    if (bad != bad) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int i = lane + 32 * j;
-        if (i >= n) continue;
-        const int64_t si = blk * kBlock + i;
-        const uint32_t r = place_hash(si, k.seed);
-        static_cast<uint8_t*>(s.m)[si] = (uint8_t)encode_m(m[j], em, ((r >> 16) << 4) | 8u);
-        static_cast<uint8_t*>(s.v)[si] = (uint8_t)encode_v(v[j], ev, ((r & 0xffffu) << 4) | 8u);
-      }
-      if (lane == 0) {
-        s.ms[blk] = (uint8_t)em;
-        s.vs[blk] = (uint8_t)ev;
+        const int sh = 8 * (j & 3);
+        const uint32_t c = code_of_bad_m(m[j], (cm[j >> 2] >> sh) & 0x7fu) | sign_m(m[j]);
+        cm[j >> 2] = (cm[j >> 2] & ~(0xffu << sh)) | c << sh;
+        cv[j >> 2] = (cv[j >> 2] & ~(0xffu << sh)) | code_of_bad_v(v[j], (cv[j >> 2] >> sh) & 0xffu) << sh;
       }
     }
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.m) + si) = make_uint2(cm[0], cm[1]);
+    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(s.v) + si) = make_uint2(cv[0], cv[1]);
+    if (lane == 0) {
+      s.ms[blk] = (uint8_t)e.m;
+      s.vs[blk] = (uint8_t)e.v;
+    }
+  } else {
+    st8(static_cast<float*>(s.m) + si, m);
+    st8(static_cast<float*>(s.v) + si, v);
+  }
+}
+
+// Starts bringing a block into L2: one 128-byte line a lane. The warps' own loads (registers for one block
+// each) are not enough bytes in flight: with the next block asked for under the present one's arithmetic
+// the loads wait for L2 instead of memory.
+template <typename G, int BITS>
+__device__ __forceinline__ void prefetch_block(const MultiTensor& t, const MultiState& s, int64_t at, int64_t blk, int lane) {
+  constexpr int kStateLine = BITS == 32 ? 32 : 128;  // values in a line
+  const char* a;
+  if (lane < 8) a = reinterpret_cast<const char*>(t.p + at) + 128 * lane;
+  else if (lane < 16) a = static_cast<const char*>(t.g) + sizeof(G) * at + 128 * (lane - 8);
+  else if (lane < 24) a = static_cast<const char*>(s.m) + BITS / 8 * (blk * kBlock) + 128 * (lane - 16);
+  else a = static_cast<const char*>(s.v) + BITS / 8 * (blk * kBlock) + 128 * (lane - 24);
+  const int lines = lane < 8 ? 8 : lane < 16 ? 2 * (int)sizeof(G) : kBlock / kStateLine;
+  if ((lane & 7) < lines) asm volatile("prefetch.global.L2 [%0];" ::"l"(a));
+}
+
+// A tensor's last block, or any block of a tensor off those borders: value by value, 32 apart.
+template <typename G, int BITS>
+__device__ __noinline__ void any_block(MultiTensor t, MultiHyper h, MultiState s, StepConst k, int64_t at, int64_t blk, int n,
+                                       int lane) {
+  const float decay = 1.f - k.lr * t.wd;
+  const float sm = BITS == 8 ? pow2_of(s.ms[blk]) : 1.f, sv = BITS == 8 ? pow2_of(s.vs[blk] + 29u) : 1.f;
+  float m[8], v[8], top_m = 0.f, top_v = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int i = lane + 32 * j;
+    m[j] = v[j] = 0.f;
+    if (i >= n) continue;
+    const int64_t si = blk * kBlock + i;
+    float p = t.p[at + i], g;
+    if constexpr (sizeof(G) == 4) g = static_cast<const float*>(t.g)[at + i];
+    else g = __bfloat162float(static_cast<const bf16*>(t.g)[at + i]);
+    if (BITS == 8) {
+      m[j] = decode_m(static_cast<const uint8_t*>(s.m)[si], sm);
+      v[j] = decode_v(static_cast<const uint8_t*>(s.v)[si], sv);
+    } else {
+      m[j] = static_cast<const float*>(s.m)[si];
+      v[j] = static_cast<const float*>(s.v)[si];
+    }
+    update(k, decay, g, p, m[j], v[j]);
+    t.p[at + i] = p;
+    if (t.p16) static_cast<bf16*>(t.p16)[at + i] = __float2bfloat16_rn(p);
+    if (h.zero_grad) {
+      if constexpr (sizeof(G) == 4) static_cast<float*>(t.g)[at + i] = 0.f;
+      else static_cast<bf16*>(t.g)[at + i] = __float2bfloat16_rn(0.f);
+    }
+    if (BITS == 32) {
+      static_cast<float*>(s.m)[si] = m[j];
+      static_cast<float*>(s.v)[si] = v[j];
+    }
+    top_m = fmaxf(top_m, fabsf(m[j]));
+    top_v = fmaxf(top_v, v[j]);
+  }
+  if (BITS == 8) {
+    const Scales e = block_scales(top_m, top_v);
+    const float um = pow2_of(254u - e.m), uv = pow2_of(254u - e.v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t si = blk * kBlock + lane + 32 * j;
+      if (lane + 32 * j >= n) continue;
+      const uint32_t r = place_hash((uint32_t)si, high_mix(si), k.seed);
+      static_cast<uint8_t*>(s.m)[si] = (uint8_t)(code_of_bad_m(m[j], encode_m(m[j], um, noise_m(r)) >> 24) | sign_m(m[j]));
+      static_cast<uint8_t*>(s.v)[si] = (uint8_t)code_of_bad_v(v[j], encode_v(v[j], uv, noise_v(r)) >> 24);
+    }
+    if (lane == 0) {
+      s.ms[blk] = (uint8_t)e.m;
+      s.vs[blk] = (uint8_t)e.v;
+    }
+  }
+}
+
+// The tensor that block w of the launch lies in, by a whole warp: 32 tensors are looked at at once, twice at
+// the most 1024. (One by one they are constant-cache misses in a row, and a copy of the places to shared
+// memory took 15 us a CTA: lanes that read different arguments wait for one another.)
+template <int CAP>
+__device__ __forceinline__ int find_tensor(const Batch<CAP>& batch, int64_t w, int lane) {
+  static_assert(CAP <= 1024, "two steps of 32");
+  const int step = (batch.count + 31) / 32;
+  int i = lane * step;
+  const int at = (__popc(__ballot_sync(0xffffffffu, i < batch.count && batch.t[min(i, CAP - 1)].first_work <= w)) - 1) * step;
+  i = at + lane;
+  return at + __popc(__ballot_sync(0xffffffffu, lane < step && i < batch.count && batch.t[min(i, CAP - 1)].first_work <= w)) - 1;
+}
+
+// A CTA takes a run of `rounds` blocks a warp, consecutive warps consecutive blocks, and ends: the memory
+// serves a few hundred short runs, handed out in order, at its copy rate (103% of it for 1.0G values of
+// 32-bit states), but a persistent grid that sweeps through all tensors together at 88%, and one whose
+// CTAs step through runs of their own at 85%.
+template <typename G, int BITS, int CAP>
+__global__ void __launch_bounds__(kThreads, 4) adamw_multi_kernel(const __grid_constant__ Batch<CAP> batch, MultiHyper h,
+                                                                  MultiState s, int blocks, int rounds, bool last_launch) {
+  constexpr int kWarps = kThreads / 32;
+  const StepConst k = step_const(h);
+  const int lane = threadIdx.x & 31;
+  int tensor = -1;
+  const int64_t stop = min((int64_t)blocks, (int64_t)(blockIdx.x + 1) * kWarps * rounds);
+  for (int64_t w = (int64_t)blockIdx.x * kWarps * rounds + (threadIdx.x >> 5); w < stop; w += kWarps) {
+    if (tensor < 0) tensor = find_tensor(batch, w, lane);
+    while (tensor + 1 < batch.count && batch.t[tensor + 1].first_work <= w) ++tensor;
+    const MultiTensor& t = batch.t[tensor];
+    const int in_t = (int)w - t.first_work;
+    const int64_t at = (int64_t)in_t * kBlock, blk = t.first_block + in_t;  // in the tensor, in the states
+    const int n = (int)min((int64_t)kBlock, t.n - at);
+    if (BITS == 8 && w + kWarps < stop && t.n - at >= (kWarps + 1) * kBlock)
+      prefetch_block<G, BITS>(t, s, at + kWarps * kBlock, blk + kWarps, lane);
+    if (t.wide && n == kBlock) whole_block<G, BITS>(t, h, s, k, at, blk, lane);
+    else any_block<G, BITS>(t, h, s, k, at, blk, n, lane);
   }
   if (!last_launch) return;
   // every CTA has read the step count; the last one to finish counts the step and re-arms the ticket
@@ -194,9 +364,11 @@ __global__ void __launch_bounds__(kThreads) adamw_multi_kernel(const __grid_cons
 
 __global__ void __launch_bounds__(kThreads) state_values_kernel(const uint8_t* m, const uint8_t* ms, const uint8_t* v,
                                                                 const uint8_t* vs, void* mo, void* vo, bool f32, int64_t n8) {
-  for (int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x; i < n8; i += (int64_t)gridDim.x * kThreads) {
+  const int64_t first = blockIdx.x * (int64_t)(4 * kThreads) + threadIdx.x;
+#pragma unroll 4
+  for (int64_t i = first; i < min(n8, first + 4 * kThreads); i += kThreads) {
     const uint2 a = reinterpret_cast<const uint2*>(m)[i], b = reinterpret_cast<const uint2*>(v)[i];
-    const float sm = pow2_of(ms[i / (kBlock / 8)]), sv = pow2_of(vs[i / (kBlock / 8)]);
+    const float sm = pow2_of(ms[i / (kBlock / 8)]), sv = pow2_of(vs[i / (kBlock / 8)] + 29u);
     float x[8], y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -234,8 +406,8 @@ __global__ void __launch_bounds__(kThreads) encode_states_kernel(const float* m,
     const uint32_t ev = scale_byte_v(__reduce_max_sync(0xffffffffu, top_v));
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      mc[blk * kBlock + lane + 32 * j] = (uint8_t)encode_m(x[j], em, 1u << 19);
-      vc[blk * kBlock + lane + 32 * j] = (uint8_t)encode_v(fabsf(y[j]), ev, 1u << 19);
+      mc[blk * kBlock + lane + 32 * j] = (uint8_t)(code_of_bad_m(x[j], encode_m(x[j], pow2_of(254u - em), 1u << 23) >> 24) | sign_m(x[j]));
+      vc[blk * kBlock + lane + 32 * j] = (uint8_t)code_of_bad_v(y[j], encode_v(fabsf(y[j]), pow2_of(254u - ev), 1u << 23) >> 24);
     }
     if (lane == 0) {
       ms[blk] = (uint8_t)em;
@@ -251,11 +423,19 @@ cudaError_t launch(const MultiTensor* t, int count, const MultiHyper& h, const M
   for (int i = 0; i < count; ++i) {
     b.t[i] = t[i];
     b.t[i].first_work = (int32_t)blocks;
+    const uintptr_t g = (uintptr_t)t[i].g, p16 = (uintptr_t)t[i].p16;
+    b.t[i].wide = (uintptr_t)t[i].p % 32 == 0 && g % (sizeof(G) == 4 ? 32 : 16) == 0 && p16 % 16 == 0;
     blocks += cdiv(t[i].n, (int64_t)kBlock);
   }
   b.count = count;
-  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(cdiv(blocks, kThreads / 32), sm_count() * 8));
-  adamw_multi_kernel<G, BITS, CAP><<<grid, kThreads, 0, st>>>(b, h, s, blocks, last);
+  LLMT_REQUIRE(blocks < 0x7fffffff, "adamw_multi: too many values for one launch");
+  // whole waves of CTAs of about `most` rounds: 8-bit blocks are small, and a CTA's start (its first loads
+  // wait for the arguments and the step's constants) is 2 us
+  constexpr int64_t most = BITS == 8 ? 32 : 4;
+  const int64_t slots = (int64_t)sm_count() * 4 * (kThreads / 32), waves = cdiv(blocks, slots * most);
+  const int rounds = (int)cdiv(blocks, slots * waves);
+  const int grid = (int)cdiv(blocks, (int64_t)rounds * (kThreads / 32));
+  adamw_multi_kernel<G, BITS, CAP><<<grid, kThreads, 0, st>>>(b, h, s, (int)blocks, rounds, last);
   return cudaGetLastError();
 }
 
@@ -285,8 +465,7 @@ cudaError_t adamw_multi(const MultiTensor* t, int count, bool grad_bf16, int bit
 cudaError_t adamw_state_values(const uint8_t* m, const uint8_t* ms, const uint8_t* v, const uint8_t* vs, void* mo, void* vo,
                                bool f32, int64_t n, cudaStream_t st) {
   if (n == 0) return cudaSuccess;
-  const int grid = (int)std::min<int64_t>(cdiv(n / 8, kThreads), sm_count() * 8);
-  state_values_kernel<<<grid, kThreads, 0, st>>>(m, ms, v, vs, mo, vo, f32, n / 8);
+  state_values_kernel<<<(unsigned)cdiv(n / 8, (int64_t)(4 * kThreads)), kThreads, 0, st>>>(m, ms, v, vs, mo, vo, f32, n / 8);
   return cudaGetLastError();
 }
 

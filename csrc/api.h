@@ -88,6 +88,7 @@ struct MultiTensor {
   int32_t first_block;  // in the states
   int32_t first_work;   // in the launch: blocks of the tensors before it (set by the launcher)
   float wd;
+  bool wide;            // on the borders that whole blocks are loaded by (set by the launcher)
 };
 struct MultiState {
   void *m, *v;        // 8 bits: codes; 32 bits: fp32

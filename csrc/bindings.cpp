@@ -342,7 +342,7 @@ struct MultiPlan {
         if (!(p16[i].is_cuda() && p16[i].get_device() == dev)) elsewhere = (int64_t)i;
       }
       t.push_back({static_cast<float*>(p[i].data_ptr()), g.data_ptr(), p16.empty() ? nullptr : p16[i].data_ptr(), numel[i],
-                   (int32_t)first_block[i], 0, (float)wd[i]});
+                   (int32_t)first_block[i], 0, (float)wd[i], false});
     }
     const int64_t n = 256 * blocks;
     const at::ScalarType dt_m = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat, dt_v = bits == 8 ? at::kByte : at::kFloat;

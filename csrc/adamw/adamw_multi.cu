@@ -272,7 +272,7 @@ __device__ __noinline__ void any_block(MultiTensor t, MultiHyper h, MultiState s
   for (int j = 0; j < 8; ++j) {
     const int i = lane + 32 * j;
     m[j] = v[j] = 0.f;
-    if (i >= n) continue;
+    if (i >= n || !LLMT_IN(at + i, at + i + 1, t.n, 611) || !LLMT_IN(blk * kBlock + i, blk * kBlock + i + 1, s.n, 612)) continue;
     const int64_t si = blk * kBlock + i;
     float p = t.p[at + i], g;
     if constexpr (sizeof(G) == 4) g = static_cast<const float*>(t.g)[at + i];
@@ -350,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_multi_kernel(const __grid_c
     const int n = (int)min((int64_t)kBlock, t.n - at);
     if (BITS == 8 && w + kWarps < stop && t.n - at >= (kWarps + 1) * kBlock)
       prefetch_block<G, BITS>(t, s, at + kWarps * kBlock, blk + kWarps, lane);
+    if (!LLMT_IN(at, at + n, t.n, 613) || !LLMT_IN(blk * kBlock, (blk + 1) * kBlock, s.n, 614)) continue;
     if (t.wide && n == kBlock) whole_block<G, BITS>(t, h, s, k, at, blk, lane);
     else any_block<G, BITS>(t, h, s, k, at, blk, n, lane);
   }

@@ -57,6 +57,7 @@ struct RopeHeads {
   void* out;
   int heads;
   int64_t isb, ist, ish, osb, ost, osh;
+  int64_t in_n, out_n;  // elements from the first to the last
 };
 struct RopeArgs {
   RopeHeads q, k;  // k.heads == 0: no k
@@ -93,6 +94,7 @@ struct MultiTensor {
 struct MultiState {
   void *m, *v;        // 8 bits: codes; 32 bits: fp32
   uint8_t *ms, *vs;   // 8 bits: one exponent byte per block
+  int64_t n;          // values of each
 };
 struct MultiHyper {
   float b1, c1, b2, c2, eps, grad_scale;  // c1 = 1 - b1, c2 = 1 - b2
@@ -200,6 +202,7 @@ struct GemmArgs {
   float* part;    // CE_FWD partials (M, n_blocks, 2)
   float* tlogit;  // CE_FWD target logits (M)
   float alpha;
+  const float* row_scale;  // CE_BWD: one more factor of each row (M), or nullptr
   void* const* peer;   // PEER_RS: device array of every rank's slot buffer (tp, rows_per_rank, ldo) bf16
   int tp_rank;         // PEER_RS: this rank's slot index in every owner's buffer
   int rows_per_rank;   // PEER_RS: output row r belongs to rank r / rows_per_rank

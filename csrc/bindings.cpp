@@ -176,7 +176,13 @@ void embedding_bwd(at::Tensor idx, at::Tensor dx, at::Tensor dW, int64_t v0) {
 
 // ---------------------------------------------------------------- rotary positions
 llmt::RopeHeads rope_heads(const at::Tensor& x, const at::Tensor& y) {
-  return {x.data_ptr(), y.data_ptr(), (int)x.size(2), x.stride(0), x.stride(1), x.stride(2), y.stride(0), y.stride(1), y.stride(2)};
+  auto extent = [](const at::Tensor& t) {
+    int64_t e = t.size(3);
+    for (int i = 0; i < 3; ++i) e += t.stride(i) * (t.size(i) - 1);
+    return t.numel() ? e : 0;
+  };
+  return {x.data_ptr(),  y.data_ptr(),  (int)x.size(2), x.stride(0), x.stride(1), x.stride(2),
+          y.stride(0), y.stride(1), y.stride(2),    extent(x),   extent(y)};
 }
 
 // Rotates q and (when given) k, (B, T, heads, hd) with unit stride along hd, into q_out / k_out:
@@ -367,7 +373,7 @@ struct MultiPlan {
                        lr.data_ptr<float>(), static_cast<const float*>(opt_ptr(grad_scale_dev, "grad_scale")),
                        step.data_ptr<int>(), reinterpret_cast<unsigned*>(ticket.data_ptr<int>()), (uint32_t)seed, zero_grad};
     llmt::MultiState s{m.data_ptr(), v.data_ptr(), static_cast<uint8_t*>(const_cast<void*>(opt_ptr(ms, "scale"))),
-                       static_cast<uint8_t*>(const_cast<void*>(opt_ptr(vs, "scale")))};
+                       static_cast<uint8_t*>(const_cast<void*>(opt_ptr(vs, "scale"))), n};
     ok(llmt::adamw_multi(t.data(), (int)t.size(), bf16, (int)bits, h, s, stream()), "adamw_multi");
     return 1;
   }
@@ -576,32 +582,38 @@ llmt::PolicyArgs policy_args(const c10::optional<at::Tensor>& old, const at::Ten
   return q;
 }
 
-// (loss, logp, coef, stats, dlogits): dlogits undefined unless `grad`.
+// (loss, logp, dlogits, coef, stats): dlogits undefined unless `grad`, the last two unless `keep`.
 std::vector<at::Tensor> policy_rows(at::Tensor logits, at::Tensor targets, c10::optional<at::Tensor> old, at::Tensor adv,
                                     c10::optional<at::Tensor> ref, c10::optional<at::Tensor> mask, double clip_lo,
-                                    double clip_hi, double kl, int64_t reduction, bool grad,
-                                    c10::optional<at::Tensor> out) {
+                                    double clip_hi, double kl, int64_t reduction, bool grad, c10::optional<at::Tensor> out,
+                                    bool keep) {
   llmt::TokenBatch a = logit_batch(logits, targets, mask);
   const llmt::PolicyArgs q = policy_args(old, adv, ref, a.B, a.T, clip_lo, clip_hi, kl, reduction);
   llmt::RowOut o{};
-  at::Tensor d;
+  at::Tensor d, coef, stats;
   if (grad && out.has_value()) d = gradient_rows(logits, out, o);
   all_on_device({{logits, "logits"}, {targets, "targets"}, {mask, "mask"}, {old, "old_logp"}, {adv, "advantages"},
                  {ref, "ref_logp"}, {out, "out"}});
   if (grad && !d.defined()) d = gradient_rows(logits, out, o);
   auto f = logits.options().dtype(at::kFloat);
   const int64_t n = (int64_t)a.B * a.T;
-  auto loss = at::empty({}, f), logp = at::empty({a.B, a.T}, f), coef = at::empty({a.B, a.T}, f),
-       stats = at::empty({a.B, a.T, 2}, f), rows = at::empty({n}, f), words = at::empty({a.B + 1}, f.dtype(at::kInt));
+  auto loss = at::empty({}, f), logp = at::empty({a.B, a.T}, f);
+  // one scratch buffer: the rows' losses, the counts and the ticket, and the slopes where nobody keeps them
+  auto scratch = at::empty({n + a.B + 1 + (keep ? 0 : n)}, f);
   o.logp = logp.data_ptr<float>();
-  o.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
   o.loss = loss.data_ptr<float>();
-  o.loss_rows = rows.data_ptr<float>();
-  o.coef = coef.data_ptr<float>();
-  o.count = words.data_ptr<int>();
+  o.loss_rows = scratch.data_ptr<float>();
+  o.count = reinterpret_cast<int*>(o.loss_rows + n);
   o.ticket = reinterpret_cast<unsigned*>(o.count + a.B);
+  o.coef = o.loss_rows + n + a.B + 1;
+  if (keep) {
+    coef = at::empty({a.B, a.T}, f);
+    stats = at::empty({a.B, a.T, 2}, f);
+    o.coef = coef.data_ptr<float>();
+    o.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
+  }
   ok(llmt::policy_rows(a, q, o, stream()), "policy_rows");
-  return {loss, logp, coef, stats, d};
+  return {loss, logp, d, coef, stats};
 }
 
 // (loss, coef) of log-probabilities.
@@ -644,42 +656,43 @@ llmt::PreferenceArgs preference_args(const c10::optional<at::Tensor>& ref, int64
   return q;
 }
 
-std::vector<at::Tensor> preference_parts(const llmt::TokenBatch& a, const llmt::PreferenceArgs& q, const at::Tensor& logp,
-                                         const at::Tensor& ticket, bool ready, llmt::RowOut& o) {
-  auto f = logp.options();
-  auto loss = at::empty({}, f), coef = at::empty({a.B, a.T}, f), rewards = at::empty({a.B}, f),
-       rows = at::empty({a.B / 2}, f);
-  o.loss = loss.data_ptr<float>();
-  o.loss_rows = rows.data_ptr<float>();
-  o.coef = coef.data_ptr<float>();
-  o.rewards = rewards.data_ptr<float>();
-  o.ticket = reinterpret_cast<unsigned*>(ticket.data_ptr<int>());
-  ok(llmt::preference_tokens(a, q, logp.data_ptr<float>(), o, ready, stream()), "preference_tokens");
-  return {loss, coef, rewards};
-}
-
-// (loss, logp, rewards, coef, stats, dlogits): dlogits undefined unless `grad`.
+// (loss, logp, rewards, dlogits, coef, stats): dlogits undefined unless `grad`, the last two unless `keep`.
 std::vector<at::Tensor> preference_rows(at::Tensor logits, at::Tensor targets, c10::optional<at::Tensor> ref,
                                         c10::optional<at::Tensor> mask, double beta, double smoothing, int64_t kind,
-                                        bool average, bool grad, c10::optional<at::Tensor> out) {
+                                        bool average, bool grad, c10::optional<at::Tensor> out, bool keep) {
   llmt::TokenBatch a = logit_batch(logits, targets, mask);
   const llmt::PreferenceArgs q = preference_args(ref, a.B, a.T, beta, smoothing, kind, average);
   llmt::RowOut o{};
-  at::Tensor d;
+  at::Tensor d, coef, stats;
   if (grad && out.has_value()) d = gradient_rows(logits, out, o);
   all_on_device({{logits, "logits"}, {targets, "targets"}, {mask, "mask"}, {ref, "ref_logp"}, {out, "out"}});
   if (grad && !d.defined()) d = gradient_rows(logits, out, o);
   auto f = logits.options().dtype(at::kFloat);
-  auto logp = at::empty({a.B, a.T}, f), stats = at::empty({a.B, a.T, 2}, f), ticket = at::empty({1}, f.dtype(at::kInt));
+  const int64_t n = (int64_t)a.B * a.T;
+  auto loss = at::empty({}, f), logp = at::empty({a.B, a.T}, f), rewards = at::empty({a.B}, f);
+  auto scratch = at::empty({(keep ? 0 : 3 * n) + a.B / 2 + 1}, f);  // stats, slopes, the pairs' losses, the ticket
+  float* p = scratch.data_ptr<float>();
+  if (keep) {
+    coef = at::empty({a.B, a.T}, f);
+    stats = at::empty({a.B, a.T, 2}, f);
+    o.coef = coef.data_ptr<float>();
+    o.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
+  } else {
+    o.stats = reinterpret_cast<float2*>(p);
+    o.coef = p + 2 * n;
+    p += 3 * n;
+  }
   o.logp = logp.data_ptr<float>();
-  o.stats = reinterpret_cast<float2*>(stats.data_ptr<float>());
-  o.ticket = reinterpret_cast<unsigned*>(ticket.data_ptr<int>());
+  o.loss = loss.data_ptr<float>();
+  o.rewards = rewards.data_ptr<float>();
+  o.loss_rows = p;
+  o.ticket = reinterpret_cast<unsigned*>(p + a.B / 2);
   llmt::RowOut first = o;
   first.dz = nullptr;
   ok(llmt::logprob_rows(a, first, stream()), "preference_rows");
-  auto r = preference_parts(a, q, logp, ticket, true, o);
+  ok(llmt::preference_tokens(a, q, o.logp, o, true, stream()), "preference_rows");
   if (grad) ok(llmt::grad_rows(a, o, false, true, stream()), "preference_rows");
-  return {r[0], logp, r[2], r[1], stats, d};
+  return {loss, logp, rewards, d, coef, stats};
 }
 
 // (loss, coef, rewards) of log-probabilities.
@@ -691,9 +704,17 @@ std::vector<at::Tensor> preference_tokens(at::Tensor logp, at::Tensor targets, i
   llmt::TokenBatch a = token_batch(targets, mask, logp.size(0), logp.size(1), V);
   const llmt::PreferenceArgs q = preference_args(ref, a.B, a.T, beta, smoothing, kind, average);
   all_on_device({{logp, "logp"}, {targets, "targets"}, {mask, "mask"}, {ref, "ref_logp"}});
-  auto ticket = at::empty({1}, logp.options().dtype(at::kInt));
+  auto f = logp.options();
+  auto loss = at::empty({}, f), coef = at::empty({a.B, a.T}, f), rewards = at::empty({a.B}, f),
+       scratch = at::empty({a.B / 2 + 1}, f);
   llmt::RowOut o{};
-  return preference_parts(a, q, logp, ticket, false, o);
+  o.loss = loss.data_ptr<float>();
+  o.loss_rows = scratch.data_ptr<float>();
+  o.coef = coef.data_ptr<float>();
+  o.rewards = rewards.data_ptr<float>();
+  o.ticket = reinterpret_cast<unsigned*>(o.loss_rows + a.B / 2);
+  ok(llmt::preference_tokens(a, q, logp.data_ptr<float>(), o, false, stream()), "preference_tokens");
+  return {loss, coef, rewards};
 }
 
 // Gradient rows coef (onehot - softmax) * grad_out from saved stats; with skip_one `out` holds
@@ -788,7 +809,8 @@ void gemm(at::Tensor a, at::Tensor b, bool ta, bool tb, int64_t epi, at::Tensor 
           c10::optional<at::Tensor> tlogit, double alpha, int64_t bn, int64_t splits, c10::optional<at::Tensor> peer,
           int64_t tp_rank, int64_t rows_per_rank, c10::optional<at::Tensor> scale_a, c10::optional<at::Tensor> scale_b,
           int64_t kind, c10::optional<at::Tensor> sfa, c10::optional<at::Tensor> sfb, c10::optional<at::Tensor> ag_src,
-          c10::optional<at::Tensor> ag_dst, c10::optional<at::Tensor> ag_flags, int64_t ag_expect, int64_t ag_tp) {
+          c10::optional<at::Tensor> ag_dst, c10::optional<at::Tensor> ag_flags, int64_t ag_expect, int64_t ag_tp,
+          c10::optional<at::Tensor> row_scale) {
   cuda2d(a, "a");
   cuda2d(b, "b");
   const bool bs = kind == 2 || kind == 3;
@@ -909,6 +931,12 @@ void gemm(at::Tensor a, at::Tensor b, bool ta, bool tb, int64_t epi, at::Tensor 
     CHECK(part->numel() >= (int64_t)M * ((N + BN - 1) / BN) * 2, "CE_FWD partial buffer too small");
   }
   if (epi == llmt::EPI_CE_BWD) CHECK(g.tgt && g.lse, "CE_BWD gemm args");
+  if (row_scale.has_value() && row_scale->defined()) {
+    CHECK(epi == llmt::EPI_CE_BWD, "row_scale goes with the CE_BWD epilogue");
+    CHECK(row_scale->scalar_type() == at::kFloat && row_scale->is_contiguous() && row_scale->numel() == M,
+          "row_scale must be ", M, " contiguous float32 values");
+    g.row_scale = static_cast<const float*>(opt_ptr(row_scale, "row_scale"));
+  }
   if (bs) {
     if (kind == 3) {
       g.scale_a = scale_a->data_ptr<float>();
@@ -1085,11 +1113,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("loss_error_code", &llmt::loss_error_code, "reset"_a = false);
   m.def("logprob_rows", &logprob_rows, "logits"_a, "targets"_a, "mask"_a = py::none());
   m.def("policy_rows", &policy_rows, "logits"_a, "targets"_a, "old"_a, "adv"_a, "ref"_a, "mask"_a, "clip_lo"_a,
-        "clip_hi"_a, "kl"_a, "reduction"_a, "grad"_a, "out"_a = py::none());
+        "clip_hi"_a, "kl"_a, "reduction"_a, "grad"_a, "out"_a = py::none(), "keep"_a = false);
   m.def("policy_tokens", &policy_tokens, "logp"_a, "targets"_a, "V"_a, "old"_a, "adv"_a, "ref"_a, "mask"_a, "clip_lo"_a,
         "clip_hi"_a, "kl"_a, "reduction"_a);
   m.def("preference_rows", &preference_rows, "logits"_a, "targets"_a, "ref"_a, "mask"_a, "beta"_a, "smoothing"_a,
-        "kind"_a, "average"_a, "grad"_a, "out"_a = py::none());
+        "kind"_a, "average"_a, "grad"_a, "out"_a = py::none(), "keep"_a = false);
   m.def("preference_tokens", &preference_tokens, "logp"_a, "targets"_a, "V"_a, "ref"_a, "mask"_a, "beta"_a, "smoothing"_a,
         "kind"_a, "average"_a);
   m.def("grad_rows", &grad_rows, "logits"_a, "targets"_a, "mask"_a, "coef"_a, "stats"_a, "grad_out"_a = py::none(),
@@ -1099,7 +1127,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "rot_cols"_a = 0, "tgt"_a = py::none(), "lse"_a = py::none(), "grad_out"_a = py::none(), "part"_a = py::none(),
         "tlogit"_a = py::none(), "alpha"_a = 1.0, "bn"_a = 0, "splits"_a = 0, "peer"_a = py::none(), "tp_rank"_a = 0, "rows_per_rank"_a = 0,
         "scale_a"_a = py::none(), "scale_b"_a = py::none(), "kind"_a = 0, "sfa"_a = py::none(), "sfb"_a = py::none(),
-        "ag_src"_a = py::none(), "ag_dst"_a = py::none(), "ag_flags"_a = py::none(), "ag_expect"_a = 0, "ag_tp"_a = 0);
+        "ag_src"_a = py::none(), "ag_dst"_a = py::none(), "ag_flags"_a = py::none(), "ag_expect"_a = 0, "ag_tp"_a = 0,
+        "row_scale"_a = py::none());
   m.def("mx_sf_bytes", &llmt::mx_sf_bytes);
   m.def("mx_quant", &mx_quant, "kind"_a, "x"_a, "q"_a, "sf"_a, "qt"_a, "sft"_a, "g"_a, "scratch"_a,
         "interleave64"_a = false, "stochastic"_a = false, "seed"_a = 0, "seed_dev"_a = py::none());

@@ -25,7 +25,7 @@
 //   ROPE       qkv GEMM: rotate-half RoPE on q/k columns while storing the packed qkv rows
 //   CE_FWD     lm head: per-row partial max / sum-exp over the tile's vocab columns and the
 //              target logit; logits are never written (reference triton_ops.py:338-364)
-//   CE_BWD     lm head recompute: dlogits = (exp(acc - lse) - onehot) * grad_out * alpha
+//   CE_BWD     lm head recompute: dlogits = (exp(acc - lse) - onehot) * grad_out * alpha [* row_scale]
 #pragma once
 #include "../common/common.cuh"
 #include "../common/sm100.cuh"
@@ -176,6 +176,7 @@ __device__ __forceinline__ void epilogue_tile(uint32_t taddr, int row, int wrow,
         t = a.tgt[row];
       }
       scale = a.alpha * (a.grad_out ? *a.grad_out : 1.f);
+      if (a.row_scale && rv) scale *= a.row_scale[row];
     }
 #pragma unroll 1
     for (int c = 0; c < BN / 64; ++c) {

@@ -33,6 +33,7 @@ namespace {
 constexpr int kMaxThreads = 256;        // of a CTA of a row: with 512, the 40 registers left to each cost 13%
 constexpr int kSliceBytes = 64 * 1024;  // of a row in a CTA's shared memory: three CTAs a SM
 constexpr int kMaxCluster = 8;
+constexpr int kFill = 4;                // CTAs a SM up to which few rows are split further
 constexpr int kPairThreads = 256;
 
 // Exponentials. Errors of one sign matter here: those of 700 tokens' log-probabilities add up in the
@@ -671,7 +672,7 @@ RowShape row_shape(const TokenBatch& a) {
   const int64_t pieces = cdiv((int64_t)a.V * e, 16) + 1, n = (int64_t)a.B * a.T;
   RowShape r{1, kMaxThreads, 0};
   while (r.ctas < kMaxCluster && pieces * 16 > (int64_t)r.ctas * kSliceBytes) r.ctas *= 2;
-  while (r.ctas < kMaxCluster && n * r.ctas * 2 <= 4 * sm_count() && pieces >= 512 * r.ctas) r.ctas *= 2;
+  while (r.ctas < kMaxCluster && n * r.ctas * 2 <= kFill * sm_count() && pieces >= 512 * r.ctas) r.ctas *= 2;
   const int64_t per = cdiv(pieces, (int64_t)r.ctas);
   r.threads = per <= 512 ? 128 : 256;
   r.bytes = (int)std::min<int64_t>(per * 16, kSliceBytes);
@@ -679,32 +680,37 @@ RowShape row_shape(const TokenBatch& a) {
 }
 
 // pdl: may start while the kernel before it in the stream, one of this file, runs.
-template <typename... K, typename... A>
-cudaError_t launch_rows(void (*kernel)(K...), const TokenBatch& a, RowShape r, int smem, bool pdl, cudaStream_t st, A&&... args) {
+template <auto KERNEL, typename... A>
+cudaError_t launch_rows(const TokenBatch& a, RowShape r, bool pdl, cudaStream_t st, A... args) {
   const int64_t n = (int64_t)a.B * a.T;
   LLMT_REQUIRE(n * r.ctas <= 0x7fffffff, "loss rows: too many tokens");
-  if (smem > 48 * 1024)
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceBytes)) return e;
+  static std::atomic<uint64_t> ready{0};  // devices on which the kernel may have its shared memory
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  if (r.bytes > 48 * 1024 && (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1))) {
+    if (cudaError_t e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, kSliceBytes)) return e;
+    if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = (unsigned)(n * r.ctas);
   cfg.blockDim = r.threads;
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = r.bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {(unsigned)r.ctas, 1, 1};
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = r.ctas > 1 ? attr : attr + 1;
-  cfg.numAttrs = (r.ctas > 1 ? 1 : 0) + (pdl ? 1 : 0);
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(args)...);
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, KERNEL, args...);
 }
 
 template <typename T, bool POLICY, bool GRAD>
 cudaError_t rows_of(const TokenBatch& a, RowShape r, const PolicyArgs& q, const RowOut& o, cudaStream_t st) {
   switch (r.threads) {
-    case 128: return launch_rows(token_rows_kernel<T, 128, POLICY, GRAD>, a, r, r.bytes, POLICY, st, a, q, o, r.ctas);
-    default: return launch_rows(token_rows_kernel<T, 256, POLICY, GRAD>, a, r, r.bytes, POLICY, st, a, q, o, r.ctas);
+    case 128: return launch_rows<token_rows_kernel<T, 128, POLICY, GRAD>>(a, r, POLICY, st, a, q, o, r.ctas);
+    default: return launch_rows<token_rows_kernel<T, 256, POLICY, GRAD>>(a, r, POLICY, st, a, q, o, r.ctas);
   }
 }
 template <bool POLICY, bool GRAD>
@@ -720,8 +726,8 @@ template <typename T>
 cudaError_t grad_rows_of(const TokenBatch& a, const RowOut& o, bool skip_one, bool pdl, cudaStream_t st) {
   const RowShape r = row_shape(a);
   switch (r.threads) {
-    case 128: return launch_rows(grad_rows_kernel<T, 128>, a, r, r.bytes, pdl, st, a, o, skip_one, r.ctas);
-    default: return launch_rows(grad_rows_kernel<T, 256>, a, r, r.bytes, pdl, st, a, o, skip_one, r.ctas);
+    case 128: return launch_rows<grad_rows_kernel<T, 128>>(a, r, pdl, st, a, o, skip_one, r.ctas);
+    default: return launch_rows<grad_rows_kernel<T, 256>>(a, r, pdl, st, a, o, skip_one, r.ctas);
   }
 }
 

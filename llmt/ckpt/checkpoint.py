@@ -50,6 +50,12 @@ def _flat_opt_state(opt, flat):
         m = _full_flat(opt.exp_avg, flat.numel, world)
         v = _full_flat(opt.exp_avg_sq, flat.numel, world)
         master = _full_flat(flat.master[opt.lo:opt.hi], flat.numel, world)
+    elif hasattr(opt, "param_states"):  # MultiAdamW: its own blocks, perhaps in 8 bits
+        m = torch.zeros(flat.numel, dtype=torch.float32, device=flat.master.device)
+        v, master = torch.zeros_like(m), flat.master
+        for (a, b), o in zip(opt.param_states(), flat.offsets):
+            m[o:o + a.numel()] = a.reshape(-1)
+            v[o:o + a.numel()] = b.reshape(-1)
     else:
         m, v, master = opt.exp_avg, opt.exp_avg_sq, flat.master
     return m, v, step, master
@@ -120,6 +126,13 @@ def load(path, model, opt=None, flat=None, sharded=False):
         model.load_state_dict(ck["model"])
     if opt is not None and ck.get("optimizer") and flat is not None:
         st = ck["optimizer"]["state"]
+        if hasattr(opt, "load_param_states"):
+            opt.load_param_states([(st[i]["exp_avg"], st[i]["exp_avg_sq"]) if i in st else None for i in range(len(flat.params))])
+            if st:
+                opt.step_t.fill_(int(float(next(iter(st.values()))["step"])))
+            opt.set_lr(ck["optimizer"]["param_groups"][0]["lr"])
+            flat.refresh_shadow()
+            return ck.get("meta", {})
         lo, hi = (opt.lo, opt.hi) if hasattr(opt, "lo") else (0, flat.numel)
         for i, (p, o) in enumerate(zip(flat.params, flat.offsets)):
             s = st.get(i)

@@ -22,6 +22,11 @@ class ModelConfig:
     rope_base: float = 10000.0
     kv_heads: int | None = None   # grouped-query attention; None means kv_heads == H
     head_dim: int | None = None   # None means d // H (set for tensor-parallel shards, where H is local)
+    # rotary positions (llmt.ops.rotary): a long-context scaling {"type": "linear" | "ntk" | "llama3" |
+    # "yarn", ...}, pairs (2j, 2j + 1) in place of (j, j + rotary_dim / 2), the part of the head that turns
+    rope_scaling: dict | None = None
+    rope_interleaved: bool = False
+    rotary_dim: int | None = None  # None means the whole head
 
     @property
     def hd(self) -> int:
@@ -30,6 +35,11 @@ class ModelConfig:
     @property
     def kvh(self) -> int:
         return self.kv_heads or self.H
+
+    @property
+    def plain_rope(self) -> bool:
+        """Half pairs over the whole head: the layout of the fused qkv epilogue and the attention backward."""
+        return not self.rope_interleaved and self.rotary_dim in (None, self.hd)
 
     @property
     def qkv_out(self) -> int:

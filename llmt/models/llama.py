@@ -63,6 +63,31 @@ def rope(x, cos, sin):
 apply_rope = rope
 
 
+def model_rope_tables(cfg: ModelConfig, T, device):
+    """The tables of a model's positions 0..T-1, each (T, rotary_dim): rope_tables for plain rotary
+    positions, those of the scaled frequencies (llmt.ops.rotary) otherwise."""
+    rd = cfg.rotary_dim or cfg.hd
+    if cfg.rope_scaling is None and rd == cfg.hd:
+        return rope_tables(T, cfg.hd, cfg.rope_base, device)
+    from llmt.ops.rotary import position_tables
+    return position_tables(T, rd, cfg.rope_base, cfg.rope_scaling, device)
+
+
+def rotate_heads(cfg: ModelConfig, x, cos, sin):
+    """`rope` in the model's layout: of the first rotary_dim values of each head, in interleaved pairs
+    where the model has them; the tables' columns j and j + rotary_dim / 2 hold the angle of pair j."""
+    if cfg.plain_rope:
+        return rope(x, cos, sin)
+    rd = cos.shape[-1]
+    turned, kept = x[..., :rd], x[..., rd:]
+    if cfg.rope_interleaved:
+        turned = torch.cat((turned[..., 0::2], turned[..., 1::2]), dim=-1)
+    turned = rope(turned, cos, sin)
+    if cfg.rope_interleaved:
+        turned = torch.stack(turned.chunk(2, dim=-1), dim=-1).flatten(-2)
+    return torch.cat((turned, kept), dim=-1)
+
+
 def act_dtype():
     """The autocast dtype in effect (the dtype normalised activations are handed on in), or None."""
     for dev in ("cuda", "cpu"):
@@ -104,7 +129,7 @@ def attention_forward(cfg: ModelConfig, w_qkv, w_o, x, cos, sin, impl="sdpa"):
     H, KV, hd = cfg.H, cfg.kvh, cfg.hd
     q, k, v = F.linear(x, w_qkv).view(B, T, H + 2 * KV, hd).split((H, KV, KV), dim=2)
     q, k, v = (t.permute(0, 2, 1, 3) for t in (q, k, v))
-    y = causal_attention(rope(q, cos, sin), rope(k, cos, sin), v, impl)
+    y = causal_attention(rotate_heads(cfg, q, cos, sin), rotate_heads(cfg, k, cos, sin), v, impl)
     return F.linear(y.permute(0, 2, 1, 3).reshape(B, T, H * hd), w_o)
 
 
@@ -222,7 +247,7 @@ class LlamaModel(nn.Module):
         self.blocks = nn.ModuleList(Block(cfg, attn_impl) for _ in range(cfg.L))
         self.norm_f = RMSNorm(cfg.d, cfg.eps)
         self.head = nn.Linear(cfg.d, cfg.vocab, bias=False)
-        cos, sin = rope_tables(max_seq, cfg.hd, cfg.rope_base, device="cpu")
+        cos, sin = model_rope_tables(cfg, max_seq, device="cpu")
         self.register_buffer("rope_cos", cos, persistent=False)
         self.register_buffer("rope_sin", sin, persistent=False)
         init_weights(self)

@@ -21,7 +21,9 @@ from llmt.models.llama import LlamaModel
 from llmt.ops import fp8 as F8
 from llmt.ops import mx as MX
 from llmt.ops import functions as Fn
+from llmt.ops import losses
 from llmt.ops import native as N
+from llmt.ops.rotary import Rotary
 
 ALIGN = 64  # elements; keeps every view 256-byte (fp32) / 128-byte (bf16) aligned
 
@@ -141,10 +143,41 @@ class NativeLlama:
         dev = model.emb.weight.device
         if dev.type != "cuda":
             raise RuntimeError("the native path runs on CUDA (sm_100a) only")
+        self.rotary = None  # the rotary layouts that the fused qkv path does not turn
+        if not model.cfg.plain_rope:
+            if linear != "bf16":
+                raise ValueError("rope_interleaved and rotary_dim go with bf16 block linears")
+            c = model.cfg
+            self.rotary = Rotary(c.hd, rotary_dim=c.rotary_dim, base=c.rope_base, interleaved=c.rope_interleaved,
+                                 scaling=c.rope_scaling, device=dev)
         self.flat = FlatParams(model, dev, pad_to=pad_to, bucket_pad=bucket_pad)
         self.ce_chunk = ce_chunk
 
     def forward(self, idx, targets):
+        h = self.hidden(idx)
+        return Fn.HeadCE.apply(h, self.model.head.weight, targets.reshape(-1), self.ce_chunk)
+
+    def token_logprobs(self, idx, targets):
+        """(B, T) fp32 log-probabilities of the targets (0 where a target is outside the vocabulary), from
+        fp32 logits that are never written; its gradient reaches the weights' main_grad. Under
+        torch.no_grad() it gives the old and reference log-probabilities of the losses below."""
+        h = self.hidden(idx)
+        return Fn.HeadLogprobs.apply(h, self.model.head.weight, targets.reshape(-1), self.ce_chunk).view(targets.shape)
+
+    def policy_loss(self, idx, targets, old_logp, advantages, **kw):
+        """llmt.ops.losses.policy_loss_tokens of this model: PolicyLoss(loss, logp)."""
+        logp = self.token_logprobs(idx, targets)
+        return losses.PolicyLoss(losses.policy_loss_tokens(logp, targets, self.cfg.vocab, old_logp, advantages, **kw), logp.detach())
+
+    def preference_loss(self, idx, targets, **kw):
+        """llmt.ops.losses.preference_loss_tokens of this model on (2 P, T) tokens, the chosen sequences
+        first: PreferenceLoss(loss, logp, rewards)."""
+        logp = self.token_logprobs(idx, targets)
+        r = losses.preference_loss_tokens(logp, targets, self.cfg.vocab, **kw)
+        return losses.PreferenceLoss(r.loss, logp.detach(), r.rewards)
+
+    def hidden(self, idx):
+        """(B T, d) bf16 input of the lm head."""
         cfg, m = self.cfg, self.model
         B, T = idx.shape
         cos = m.rope_cos[:T].contiguous()
@@ -164,8 +197,7 @@ class NativeLlama:
                 a, r = self._block(blk, a, r, cos, sin, B, T)
             if self.nvtx:
                 torch.cuda.nvtx.range_pop()
-        h = Fn.FinalNormFn.apply(a, r, m.norm_f.weight, cfg.eps)
-        return Fn.HeadCE.apply(h, m.head.weight, targets.reshape(-1), self.ce_chunk)
+        return Fn.FinalNormFn.apply(a, r, m.norm_f.weight, cfg.eps)
 
     def _block(self, blk, a, r, cos, sin, B, T):
         cfg = self.cfg
@@ -184,7 +216,10 @@ class NativeLlama:
             att = F8.LinearFP8.apply(o, blk.attn.wo.weight)
             n2, s2 = Fn.AddRMSNormFn.apply(att, s1, blk.norm2.weight, cfg.eps)
             return F8.SwiGLUMLPFP8.apply(n2, blk.mlp.w1.weight, blk.mlp.w2.weight, cfg.ffn), s2
-        o = Fn.QKVAttention.apply(n1, blk.attn.qkv.weight, cos, sin, B, T, cfg.H, cfg.kvh, cfg.hd)
+        if self.rotary is not None:
+            o = Fn.QKVAttentionRotary.apply(n1, blk.attn.qkv.weight, self.rotary, B, T, cfg.H, cfg.kvh, cfg.hd)
+        else:
+            o = Fn.QKVAttention.apply(n1, blk.attn.qkv.weight, cos, sin, B, T, cfg.H, cfg.kvh, cfg.hd)
         att = Fn.Linear.apply(o, blk.attn.wo.weight)
         n2, s2 = Fn.AddRMSNormFn.apply(att, s1, blk.norm2.weight, cfg.eps)
         return Fn.SwiGLUMLP.apply(n2, blk.mlp.w1.weight, blk.mlp.w2.weight, cfg.ffn), s2

@@ -15,6 +15,9 @@ Regions (reference equivalents in bench_train.py / kernels/triton_ops.py):
   Linear         y = x W^T (wo)                                  bench_train.py:150
   SwiGLUMLP      w1||w3 GEMM (+SwiGLU epilogue) -> w2 GEMM       bench_train.py:153-163
   HeadCE         lm head + cross entropy, logits never written   triton_ops.py:367-405
+Post-training regions without a counterpart there:
+  QKVAttentionRotary   QKVAttention for interleaved or partial rotary positions
+  HeadLogprobs         lm head -> log-probabilities of the targets (policy and preference losses)
 """
 from __future__ import annotations
 
@@ -183,6 +186,39 @@ class QKVAttention(torch.autograd.Function):
         return dx, None, None, None, None, None, None, None, None
 
 
+class QKVAttentionRotary(torch.autograd.Function):
+    """QKVAttention for the rotary layouts that the qkv epilogue and the attention backward do not turn
+    (interleaved pairs, a part of the head): the rotation is its own kernel, in place on the packed
+    rows, forward after the plain qkv GEMM and backward on dqkv (the attention backward's own
+    rotation is given the angle zero)."""
+
+    @staticmethod
+    def forward(ctx, x, w, rotary, B, T, H, KV, hd):
+        qkv = N.gemm(x, w.w16, ta=False, tb=True)
+        heads = qkv.view(B, T, H + 2 * KV, hd)
+        q, k = heads[:, :, :H], heads[:, :, H:H + KV]
+        rotary.rotate(q, k, q_out=q, k_out=k)
+        o, lse = N.flash_attn_fwd(qkv, B, T, H, KV, hd, causal=True)
+        ctx.save_for_backward(x, qkv, o, lse)
+        ctx.w, ctx.rotary = w, rotary
+        ctx.dims = (B, T, H, KV, hd)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        x, qkv, o, lse = ctx.saved_tensors
+        B, T, H, KV, hd = ctx.dims
+        w = ctx.w
+        one = torch.ones((T, hd), dtype=torch.float32, device=qkv.device)
+        dqkv = N.flash_attn_bwd(do.contiguous(), qkv, o, lse, one, torch.zeros_like(one), B, T, H, KV, hd, causal=True)
+        heads = dqkv.view(B, T, H + 2 * KV, hd)
+        dq, dk = heads[:, :, :H], heads[:, :, H:H + KV]
+        ctx.rotary.rotate(dq, dk, inverse=True, q_out=dq, k_out=dk)
+        dx = N.gemm(dqkv, w.w16, ta=False, tb=False)
+        _wgrad(dqkv, x, w)
+        return dx, None, None, None, None, None, None, None
+
+
 class Linear(torch.autograd.Function):
     """y = x W^T with bf16 operands; W's fp32 gradient goes to W.main_grad."""
 
@@ -320,6 +356,39 @@ class HeadCE(torch.autograd.Function):
             c1 = min(n, c0 + chunk)
             hc = h[c0:c1]
             dl = N.gemm_ce_bwd(hc, w.w16, targets[c0:c1], lse[c0:c1], g, 1.0 / n)
+            N.gemm(dl, w.w16, ta=False, tb=False, out=dh[c0:c1])
+            if c0 == 0:
+                wgrad_into(dl, hc, w.main_grad)
+            else:
+                N.gemm(dl, hc, ta=True, tb=False, out=w.main_grad, accumulate=True)
+        return dh, None, None, None
+
+
+class HeadLogprobs(torch.autograd.Function):
+    """Log-probabilities (N,) fp32 of the targets under the lm head, logits never written: the fused head GEMM's
+    log-sum-exp and target logit (from its fp32 accumulators), and in the backward its recomputed
+    tiles as bf16 rows of -g (softmax - onehot), g the incoming gradient of each row. A target outside the
+    vocabulary gives 0 and no gradient."""
+
+    @staticmethod
+    def forward(ctx, h, w, targets, chunk):
+        lse, _, tl = N.gemm_ce_fwd(h, w.w16, targets, return_target_logit=True)
+        counts = (targets >= 0) & (targets < w.shape[0])
+        ctx.save_for_backward(h, targets, lse, counts)
+        ctx.w, ctx.chunk = w, chunk
+        return torch.where(counts, tl - lse, torch.zeros_like(lse))
+
+    @staticmethod
+    def backward(ctx, g):
+        h, targets, lse, counts = ctx.saved_tensors
+        w, chunk = ctx.w, ctx.chunk
+        n = h.shape[0]
+        rows = torch.where(counts, -g, torch.zeros_like(g)).contiguous()
+        dh = torch.empty_like(h)
+        for c0 in range(0, n, chunk):
+            c1 = min(n, c0 + chunk)
+            hc = h[c0:c1]
+            dl = N.gemm_ce_bwd(hc, w.w16, targets[c0:c1], lse[c0:c1], None, 1.0, row_scale=rows[c0:c1])
             N.gemm(dl, w.w16, ta=False, tb=False, out=dh[c0:c1])
             if c0 == 0:
                 wgrad_into(dl, hc, w.main_grad)

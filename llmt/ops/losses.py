@@ -70,10 +70,10 @@ def logprob_rows(logits, targets, mask=None):
     return N.ext().logprob_rows(logits.detach(), targets, mask)[0]
 
 
-def _policy_rows(logits, targets, old_logp, advantages, ref_logp, mask, clip, kl_coef, reduction, grad, out=None):
+def _policy_rows(logits, targets, old_logp, advantages, ref_logp, mask, clip, kl_coef, reduction, grad, out=None, keep=False):
     lo, hi = _clip(clip)
     return N.ext().policy_rows(logits.detach(), targets, old_logp, advantages, ref_logp, mask, lo, hi, float(kl_coef),
-                               _choice(REDUCTIONS, reduction, "reduction"), bool(grad), out)
+                               _choice(REDUCTIONS, reduction, "reduction"), bool(grad), out, keep)
 
 
 def policy_loss_rows(logits, targets, old_logp, advantages, ref_logp=None, mask=None, clip=(0.2, 0.2), kl_coef=0.0,
@@ -87,7 +87,7 @@ def policy_loss_rows(logits, targets, old_logp, advantages, ref_logp=None, mask=
     old_logp None takes the current log-probabilities (the first step on a batch); advantages are
     (B, T) or broadcast to it, (B, 1) for one per sequence. `out` takes the gradient; it may be the
     logits themselves. Returns PolicyRows(loss, logp, dlogits)."""
-    loss, logp, _, _, d = _policy_rows(logits, targets, old_logp, advantages, ref_logp, mask, clip, kl_coef, reduction,
+    loss, logp, d, _, _ = _policy_rows(logits, targets, old_logp, advantages, ref_logp, mask, clip, kl_coef, reduction,
                                        grad, out)
     return PolicyRows(loss, logp, d if grad else None)
 
@@ -103,7 +103,7 @@ def preference_loss_rows(logits, targets, ref_logp=None, mask=None, beta=0.1, ki
         hinge:   max(0, 1 - beta D)
         ipo:     (D - 1 / (2 beta))^2
     averaged over pairs. Returns PreferenceRows(loss, logp, rewards = beta * gains (2 P), dlogits)."""
-    loss, logp, rewards, _, _, d = N.ext().preference_rows(
+    loss, logp, rewards, d, _, _ = N.ext().preference_rows(
         logits.detach(), targets, ref_logp, mask, float(beta), float(label_smoothing), _choice(KINDS, kind, "kind"), bool(average),
         bool(grad), out)
     return PreferenceRows(loss, logp, rewards, d if grad else None)
@@ -117,8 +117,8 @@ class _PolicyRowsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, old_logp, advantages, ref_logp, mask, clip, kl_coef, reduction):
         want = ctx.needs_input_grad[0]
-        loss, logp, coef, stats, d = _policy_rows(logits, targets, old_logp, advantages, ref_logp, mask, clip, kl_coef,
-                                                  reduction, want)
+        loss, logp, d, coef, stats = _policy_rows(logits, targets, old_logp, advantages, ref_logp, mask, clip, kl_coef,
+                                                  reduction, want, keep=want)
         if want:
             ctx.save_for_backward(logits, targets, mask, coef, stats)
             ctx.ready = d
@@ -136,9 +136,9 @@ class _PolicyRowsFn(torch.autograd.Function):
 class _PreferenceRowsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, ref_logp, mask, beta, kind, label_smoothing, average):
-        loss, logp, rewards, coef, stats, _ = N.ext().preference_rows(
+        loss, logp, rewards, _, coef, stats = N.ext().preference_rows(
             logits.detach(), targets, ref_logp, mask, float(beta), float(label_smoothing), _choice(KINDS, kind, "kind"),
-            bool(average), False, None)
+            bool(average), False, None, True)
         ctx.save_for_backward(logits, targets, mask, coef, stats)
         ctx.mark_non_differentiable(logp, rewards)
         return loss, logp, rewards

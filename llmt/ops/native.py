@@ -200,12 +200,14 @@ def gemm_ce_fwd(h, w, targets, bn=256, return_target_logit=False):
     return (lse, loss, tl) if return_target_logit else (lse, loss)
 
 
-def gemm_ce_bwd(h, w, targets, lse, grad_out, scale, out=None, bn=0):
-    """Recomputed logit tiles -> dlogits = (softmax - onehot) * grad_out * scale, bf16 (M, V)."""
+def gemm_ce_bwd(h, w, targets, lse, grad_out, scale, out=None, bn=0, row_scale=None):
+    """Recomputed logit tiles -> dlogits = (softmax - onehot) * grad_out * scale, bf16 (M, V); row_scale:
+    (M,) fp32, one more factor of each row."""
     M, V = h.shape[0], w.shape[0]
     if out is None:
         out = torch.empty((M, V), dtype=torch.bfloat16, device=h.device)
-    ext().gemm(h, w, False, True, EPI_CE_BWD, out, tgt=targets, lse=lse, grad_out=grad_out, alpha=scale, bn=bn)
+    ext().gemm(h, w, False, True, EPI_CE_BWD, out, tgt=targets, lse=lse, grad_out=grad_out, alpha=scale, bn=bn,
+               row_scale=row_scale)
     return out
 
 

@@ -79,13 +79,20 @@ def frequencies(rotary_dim, base=10000.0, scaling=None):
     return w, 1.0
 
 
+def position_tables(T, rotary_dim, base=10000.0, scaling=None, device="cpu"):
+    """(cos, sin), each (T, rotary_dim) fp32 with both halves alike, for positions 0 .. T - 1; angles in fp64."""
+    inv_freq, factor = frequencies(rotary_dim, base, scaling)
+    angle = (torch.arange(T, dtype=torch.float64)[:, None] * inv_freq).repeat(1, 2)
+    return (angle.cos() * factor).float().to(device), (angle.sin() * factor).float().to(device)
+
+
 class Rotary:
     def __init__(self, head_dim, rotary_dim=None, base=10000.0, interleaved=False, scaling=None, device="cuda"):
         self.head_dim = int(head_dim)
         self.rotary_dim = int(rotary_dim) if rotary_dim is not None else self.head_dim
         if not 0 < self.rotary_dim <= self.head_dim:
             raise ValueError(f"rotary_dim must be in (0, head_dim = {self.head_dim}], not {self.rotary_dim}")
-        self.interleaved = bool(interleaved)
+        self.interleaved, self.base, self.scaling = bool(interleaved), base, scaling
         self.inv_freq, self.factor = frequencies(self.rotary_dim, base, scaling)
         digit = torch.cat([torch.arange(1024), torch.arange(1024) << 10, torch.arange(2048) << 20]).double()
         angle = digit[:, None] * self.inv_freq
@@ -96,9 +103,7 @@ class Rotary:
     def tables(self, T, device=None):
         """(cos, sin), each (T, rotary_dim) fp32 with both halves alike, for positions 0 .. T - 1: the
         tables of the fused qkv path (which rotates half pairs of whole heads)."""
-        angle = (torch.arange(T, dtype=torch.float64)[:, None] * self.inv_freq).repeat(1, 2)
-        dev = self.table.device if device is None else device
-        return (angle.cos() * self.factor).float().to(dev), (angle.sin() * self.factor).float().to(dev)
+        return position_tables(T, self.rotary_dim, self.base, self.scaling, self.table.device if device is None else device)
 
     def rotate(self, q, k=None, positions=None, inverse=False, q_out=None, k_out=None):
         """(q, k) turned to their positions: q (B, T, H, head_dim), k (B, T, KV, head_dim) or None, bf16 /

@@ -71,7 +71,8 @@ def check_device_errors(reset: bool = True):
     """Raise DeviceWaitTimeout if any bounded device-side wait gave up since the last check."""
     from llmt.ops import native as N
     C = N.ext()
-    codes = {"gemm": N.gemm_error_code(reset), "attention": N.attn_error_code(reset), "dp": C.dp_error_code(reset)}
+    codes = {"gemm": N.gemm_error_code(reset), "attention": N.attn_error_code(reset), "dp": C.dp_error_code(reset),
+             "loss": N.loss_error_code(reset)}
     bad = {k: v for k, v in codes.items() if v}
     if bad:
         msg = "; ".join(f"{k}: {_phase(k, v)}" for k, v in bad.items())

@@ -29,7 +29,7 @@ import torch.nn.functional as F
 
 from llmt.config import ModelConfig
 from llmt.export.trace import schedule_1f1b
-from llmt.models.llama import Block, RMSNorm, build_model, rope_tables
+from llmt.models.llama import Block, RMSNorm, build_model, model_rope_tables
 from llmt.parallel.collectives import gather_rows, scatter_rows
 
 
@@ -53,7 +53,9 @@ class StageModel(nn.Module):
         self.emb = nn.Embedding(cfg.vocab, cfg.d) if first else None
         self.norm_f = RMSNorm(cfg.d, cfg.eps) if last else None
         self.head = nn.Linear(cfg.d, cfg.vocab, bias=False) if last else None
-        cos, sin = rope_tables(max_seq, cfg.hd, cfg.rope_base, device="cpu")
+        if not cfg.plain_rope:
+            raise ValueError("pipeline stages rotate half pairs of whole heads: rope_interleaved and rotary_dim are single-GPU options")
+        cos, sin = model_rope_tables(cfg, max_seq, device="cpu")
         self.register_buffer("rope_cos", cos, persistent=False)
         self.register_buffer("rope_sin", sin, persistent=False)
         for m in self.modules():

@@ -45,6 +45,8 @@ from llmt.parallel.collectives import gather_rows, scatter_rows
 
 
 def local_config(cfg: ModelConfig, tp: int) -> ModelConfig:
+    if not cfg.plain_rope:
+        raise ValueError("tensor-parallel shards rotate half pairs of whole heads: rope_interleaved and rotary_dim are single-GPU options")
     for name, v in (("heads", cfg.H), ("kv heads", cfg.kvh), ("ffn", cfg.ffn), ("vocab", cfg.vocab)):
         if v % tp:
             raise ValueError(f"tensor parallel {tp} does not divide {name} = {v}")

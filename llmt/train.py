@@ -22,16 +22,22 @@ from llmt.models.native import NativeLlama
 from llmt.ops import functions as Fn
 from llmt.ops import native
 from llmt.optim.adamw import FusedAdamW
+from llmt.optim.multi import MultiAdamW
 
 
 class Trainer:
     """tp_group: tensor + sequence parallel group (the model is then this rank's shard, see
-    llmt.parallel.tp); dp: a DataParallel over the data-parallel group (ZeRO-1)."""
+    llmt.parallel.tp); dp: a DataParallel over the data-parallel group (ZeRO-1); optimizer: "adamw" (fp32
+    states) or "adamw8" (8-bit states, llmt.optim.multi: 2 bytes a parameter in place of 8)."""
 
     def __init__(self, cfg: ModelConfig, batch: int, seq: int, device="cuda", seed: int = 0, lr: float = 3e-4,
                  cuda_graph: bool = True, microbatches: int = 1, dp=None, ce_chunk: int = 8192, ckpt: bool = False,
                  tp_group=None, init: str = "full", nvtx: bool = False, linear: str = "bf16",
-                 first_write: bool = True):
+                 first_write: bool = True, optimizer: str = "adamw"):
+        if optimizer not in ("adamw", "adamw8"):
+            raise ValueError(f"optimizer must be adamw or adamw8, not {optimizer!r}")
+        if optimizer == "adamw8" and (dp is not None or tp_group is not None):
+            raise ValueError("adamw8 is a single-GPU optimizer: the data-parallel step shards its own, tensor parallelism is not tested with it")
         self.cfg, self.batch, self.seq = cfg, batch, seq
         self.linear = linear
         self.nvtx = nvtx  # NVTX ranges forward / backward / optimizer per step (eager steps; reference --nvtx)
@@ -63,6 +69,9 @@ class Trainer:
         if dp is not None:
             self.opt = dp.make_optimizer(flat, lr=lr)
             dp.zero_grads = not self.first_write
+        elif optimizer == "adamw8":
+            self.opt = MultiAdamW(flat.params, [p.w16 for p in flat.params], [p.main_grad for p in flat.params], lr=lr,
+                                  state_bits=8, seed=seed, zero_grad=not self.first_write)
         else:
             self.opt = FusedAdamW(flat.master, flat.grad, flat.shadow, lr=lr, zero_grad=not self.first_write)
         mb = batch // microbatches

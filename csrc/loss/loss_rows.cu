@@ -31,7 +31,8 @@ namespace llmt {
 namespace {
 
 constexpr int kMaxThreads = 256;        // of a CTA of a row: with 512, the 40 registers left to each cost 13%
-constexpr int kSliceBytes = 64 * 1024;  // of a row in a CTA's shared memory: three CTAs a SM
+constexpr int kTileBytes = 32 * 1024;   // of a row, two in a CTA's shared memory, three CTAs a SM
+constexpr int kSliceBytes = 2 * kTileBytes;
 constexpr int kMaxCluster = 8;
 constexpr int kFill = 4;                // CTAs a SM up to which few rows are split further
 constexpr int kPairThreads = 256;
@@ -281,7 +282,7 @@ struct alignas(8) MaxSum {  // written to other CTAs as one 8-byte vector
 // The pieces of a CTA of a row's cluster: [lo, hi), in tiles of the shared memory's size.
 template <typename T, int THREADS>
 struct Slice {
-  static constexpr int kTile = kSliceBytes / 16;
+  static constexpr int kTile = kTileBytes / 16;
   int lo, hi;
   __device__ Slice(const RowView<T>& v, int rank, int ctas) {
     const int per = (v.pieces + ctas - 1) / ctas;
@@ -389,14 +390,42 @@ __device__ __forceinline__ float row_logp(float zy, MaxSum r) {
 
 __device__ int g_error = 0;  // 1: a copy did not arrive within its wait's limit (the results are void)
 
-// All threads wait for a tile. One warp polls while the others rest at the CTA's barrier: sixteen polling
-// warps took more of the SM's issue slots than the row's arithmetic (21.5 instructions a value against 9.5).
-// After a wait that ran out, one more for the copy: the CTA must not end under it.
-__device__ __forceinline__ void wait_tile(uint64_t* bar, uint32_t parity) {
-  if (threadIdx.x < 32 && !sm100::wait_bar(bar, parity, &g_error, 1)) sm100::wait_bar(bar, parity, &g_error, 1);
-  __syncthreads();
-  sm100::bar_try_wait(bar, parity);  // done: each thread sees the copy for itself
-}
+// A row's tiles in a CTA's two buffers, tile t in buffer t & 1: the next one is on its way while one is worked on.
+// One warp polls for a copy while the others rest at the CTA's barrier: eight polling warps take issue slots
+// from the other rows' arithmetic. After a wait that ran out, one more for the copy: the CTA must not end under it.
+template <typename T, int THREADS>
+struct Tiles {
+  const RowView<T>& in;
+  const Slice<T, THREADS>& s;
+  uint4* buf;
+  uint64_t* bar;
+  uint32_t phase = 0;  // bit b: of buffer b's barrier
+  __device__ __forceinline__ void init() {
+    if (threadIdx.x == 0) {
+      sm100::bar_init(&bar[0], 1);
+      sm100::bar_init(&bar[1], 1);
+      sm100::fence_barrier_init();
+      sm100::fence_proxy_async_smem();
+    }
+  }
+  __device__ __forceinline__ uint4* at(int tile) const { return buf + (tile & 1) * Slice<T, THREADS>::kTile; }
+  __device__ __forceinline__ void fill(int tile) const { fill_tile(in, s, tile, at(tile), &bar[tile & 1]); }
+  // Into the buffer of a tile that the CTA has read.
+  __device__ __forceinline__ void refill(int tile) const {
+    __syncthreads();
+    if (threadIdx.x == 0) sm100::fence_proxy_async_smem();
+    fill(tile);
+  }
+  __device__ __forceinline__ const uint4* wait(int tile) {
+    const int b = tile & 1;
+    const uint32_t parity = phase >> b & 1;
+    if (threadIdx.x < 32 && !sm100::wait_bar(&bar[b], parity, &g_error, 1)) sm100::wait_bar(&bar[b], parity, &g_error, 1);
+    __syncthreads();
+    sm100::bar_try_wait(&bar[b], parity);  // done: each thread sees the copy for itself
+    phase ^= 1u << b;
+    return at(tile);
+  }
+};
 
 // One cluster per row: its maximum, sum and log-probability; with POLICY the loss and slope of its
 // token, with GRAD also the row of the gradient. The row lies in shared memory from its one read to its
@@ -407,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(Toke
   extern __shared__ uint4 buf[];
   __shared__ MaxSum part[kMaxCluster * kWarps];
   __shared__ float s_row[3];
-  __shared__ uint64_t bar;
+  __shared__ uint64_t bar[2];
   const int64_t n = blockIdx.x / ctas;
   const int rank = (int)(blockIdx.x % ctas), warp = (int)threadIdx.x >> 5, lane = (int)threadIdx.x & 31;
   const int b = (int)(n / a.T), t = (int)(n % a.T);
@@ -428,12 +457,10 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(Toke
   } else {
     const Slice<T, THREADS> s(in, rank, ctas);
     const int tiles = s.tiles();
-    if (threadIdx.x == 0) {
-      sm100::bar_init(&bar, 1);
-      sm100::fence_barrier_init();
-      sm100::fence_proxy_async_smem();
-    }
-    fill_tile(in, s, 0, buf, &bar);  // thread 0 made the barrier
+    Tiles<T, THREADS> held{in, s, buf, bar};
+    held.init();
+    held.fill(0);  // thread 0 made the barriers
+    if (tiles > 1) held.fill(1);
     // (a CTA's shared memory may be written by others once it has begun)
     if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     // what the token's loss needs, while the row is on its way
@@ -445,21 +472,14 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(Toke
       pdl_wait();  // the counts
       weight = token_weight(o.count, a.B, b, q.reduction);
     }
-    uint32_t parity = 0;
     MaxSum ms = {-INFINITY, 0.f};
     for (int tile = 0; tile < tiles; ++tile) {
-      if (tile > 0) {
-        __syncthreads();  // the tile before has been read
-        if (threadIdx.x == 0) sm100::fence_proxy_async_smem();
-        fill_tile(in, s, tile, buf, &bar);
-      }
-      wait_tile(&bar, parity);
-      parity ^= 1;
+      const uint4* const x = held.wait(tile);
       const int count = s.end(tile) - s.begin(tile);
       float m = ms.m;
 #pragma unroll 4
       for (int i = threadIdx.x; i < count; i += THREADS) {
-        const uint4 v = buf[i];
+        const uint4 v = x[i];
         m = piece_max(Piece<T>{{v.x, v.y, v.z, v.w}}, m);
       }
 #pragma unroll
@@ -468,13 +488,14 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(Toke
       float2 sum = make_float2(ms.s == 0.f ? 0.f : ms.s * exp_(ms.m - at), 0.f);
 #pragma unroll 4
       for (int i = threadIdx.x; i < count; i += THREADS) {
-        const uint4 v = buf[i];
-        const Piece<T> x = {{v.x, v.y, v.z, v.w}};
+        const uint4 v = x[i];
+        const Piece<T> f = {{v.x, v.y, v.z, v.w}};
 #pragma unroll
-        for (int h = 0; h < Piece<T>::N / 2; ++h) sum = add_exp(pair_of(x, h), make_float2(-at, -at), sum);
+        for (int h = 0; h < Piece<T>::N / 2; ++h) sum = add_exp(pair_of(f, h), make_float2(-at, -at), sum);
       }
       ms.m = m;
       ms.s = sum.x + sum.y;
+      if (tile + 2 < tiles) held.refill(tile + 2);
     }
     ms.s = warp_sum(ms.s);
     // every warp's pair to every CTA of the cluster
@@ -514,17 +535,12 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(Toke
       if (c == 0.f) {
         zero_row<T, THREADS>(out, rank, ctas);
       } else {
-        for (int tile = tiles - 1; tile >= 0; --tile) {  // the last one is still there
-          if (tile != tiles - 1) {
-            __syncthreads();
-            if (threadIdx.x == 0) sm100::fence_proxy_async_smem();
-            fill_tile(in, s, tile, buf, &bar);
-            wait_tile(&bar, parity);
-            parity ^= 1;
-          }
+        for (int tile = tiles - 1; tile >= 0; --tile) {  // the last two are still there, the others in L2
+          const uint4* const x = tile + 2 < tiles ? held.wait(tile) : held.at(tile);
           const int first = s.begin(tile);
           store_pieces<T, THREADS>(out, in, first, s.end(tile),
-                                   [&](int i) { return gradient_piece<T>(buf[i - first], m, make_float2(k, k)); });
+                                   [&](int i) { return gradient_piece<T>(x[i - first], m, make_float2(k, k)); });
+          if (tile >= 2) held.refill(tile - 2);
         }
         if (s.owns(((int)y + in.off) / Piece<T>::N)) gradient_target(out, (int)y, zy, m, k, c);
       }
@@ -548,7 +564,7 @@ __global__ void __launch_bounds__(1024) sum_rows_kernel(const float* x, int64_t 
 template <typename T, int THREADS>
 __global__ void __launch_bounds__(THREADS, 768 / THREADS) grad_rows_kernel(TokenBatch a, RowOut o, bool skip_one, int ctas) {
   extern __shared__ uint4 buf[];
-  __shared__ uint64_t bar;
+  __shared__ uint64_t bar[2];
   pdl_trigger();
   const float g = o.grad_out ? *o.grad_out : 1.f;
   if (skip_one && g == 1.f) return;
@@ -564,34 +580,31 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) grad_rows_kernel(Token
   const int tiles = s.tiles();
   const bool mine = counts && s.owns(((int)y + in.off) / Piece<T>::N);
   const float zy = mine ? to_f(in.p[y]) : 0.f;
-  if (threadIdx.x == 0) {
-    sm100::bar_init(&bar, 1);
-    sm100::fence_barrier_init();
-    sm100::fence_proxy_async_smem();
+  Tiles<T, THREADS> held{in, s, buf, bar};
+  held.init();
+  // the copies run while the slopes are waited for
+  if (counts) {
+    held.fill(tiles - 1);
+    if (tiles > 1) held.fill(tiles - 2);
   }
-  // the copy runs while the slopes are waited for, unless the token has none
-  if (counts) fill_tile(in, s, tiles - 1, buf, &bar);
   pdl_wait();
   const float c = o.coef[n] * g;
-  if (counts) wait_tile(&bar, 0);
   if (!counts || c == 0.f) {
+    if (counts) {  // a token without a slope: its copies must not outlive the CTA
+      held.wait(tiles - 1);
+      if (tiles > 1) held.wait(tiles - 2);
+    }
     zero_row<T, THREADS>(out, rank, ctas);
     return;
   }
   const float2 ms = o.stats[n];
   const float k = -c / ms.y;
-  uint32_t parity = 1;
   for (int tile = tiles - 1; tile >= 0; --tile) {
+    const uint4* const x = held.wait(tile);
     const int first = s.begin(tile);
-    if (tile != tiles - 1) {
-      __syncthreads();
-      if (threadIdx.x == 0) sm100::fence_proxy_async_smem();
-      fill_tile(in, s, tile, buf, &bar);
-      wait_tile(&bar, parity);
-      parity ^= 1;
-    }
     store_pieces<T, THREADS>(out, in, first, s.end(tile),
-                             [&](int i) { return gradient_piece<T>(buf[i - first], ms.x, make_float2(k, k)); });
+                             [&](int i) { return gradient_piece<T>(x[i - first], ms.x, make_float2(k, k)); });
+    if (tile >= 2) held.refill(tile - 2);
   }
   if (mine) gradient_target(out, (int)y, zy, ms.x, k, c);
 }
@@ -662,8 +675,8 @@ __global__ void __launch_bounds__(kPairThreads) preference_kernel(TokenBatch a, 
   last_one_sums(o.ticket, 1, P, o.loss_rows, P, 1.f / (float)P, o.loss);
 }
 
-// CTAs and threads for a row: as many CTAs as hold it (64 KB each), and more while the rows would leave
-// SMs without work; fewer threads for short rows.
+// One CTA a row where there are enough of them for every SM, each streaming its row's tiles; few rows are
+// split over clusters.
 struct RowShape {
   int ctas, threads, bytes;
 };
@@ -671,11 +684,10 @@ RowShape row_shape(const TokenBatch& a) {
   const int e = a.dtype == 2 ? 4 : 2;
   const int64_t pieces = cdiv((int64_t)a.V * e, 16) + 1, n = (int64_t)a.B * a.T;
   RowShape r{1, kMaxThreads, 0};
-  while (r.ctas < kMaxCluster && pieces * 16 > (int64_t)r.ctas * kSliceBytes) r.ctas *= 2;
   while (r.ctas < kMaxCluster && n * r.ctas * 2 <= kFill * sm_count() && pieces >= 512 * r.ctas) r.ctas *= 2;
   const int64_t per = cdiv(pieces, (int64_t)r.ctas);
   r.threads = per <= 512 ? 128 : 256;
-  r.bytes = (int)std::min<int64_t>(per * 16, kSliceBytes);
+  r.bytes = (int)(per * 16 <= kTileBytes ? per * 16 : kSliceBytes);
   return r;
 }
 

@@ -15,11 +15,16 @@
 // A token counts where its mask is set and its target is an id of the vocabulary; the logits of
 // every other row are not read (they may hold anything), and its gradient is zero.
 //
-// A row is held in the shared memory of a cluster of 1 to 8 CTAs, each a run of its 16-byte pieces: the
-// logits are read once, the maximum and sum of each warp are exchanged through distributed shared
-// memory, and the gradient is computed from what is held. Rows that do not fit (over 512 KB) are
-// read again. Sums, maxima and slopes are fp32, the sums over tokens fp64, and the gradient is
-// rounded once, to the logits' type. No atomics touch a result: equal inputs give equal bits.
+// Bound by memory: the logits of the rows that count once, all of the gradient once. A CTA streams its row
+// through two 32 KB tiles of shared memory by bulk copies, summing one while the next arrives, and
+// goes back from the last tile to the first for the gradient: the last two are still there, the others are
+// read again from L2 or memory. Three CTAs of 256 threads a SM work on different rows. (2 x 32 KB and 3 CTAs
+// 337 us for 4 x 1024 x 128256 bf16; 3 x 32 KB and 2 CTAs 342, 4 x 16 KB 363, 2 x 24 KB and 4 CTAs 355; a row held
+// by a cluster of 64 KB slices, read once but waited for as a whole, 410; gradients stored without the streaming
+// hint 357.) Where there are few rows a cluster of up to 8 CTAs shares one, and exchanges the maximum and
+// sum of each warp through distributed shared memory. Sums, maxima and slopes are fp32, the sums over
+// tokens fp64, and the gradient is rounded once, to the logits' type. No atomics touch a result: equal inputs
+// give equal bits.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -297,16 +302,20 @@ struct Slice {
 };
 
 // Brings a tile into shared memory: its whole pieces in one bulk copy, the row's ragged ends by their
-// threads. Complete after wait_tile.
+// threads. Complete after Tiles::wait. last: the tile is not read again (its lines leave L2 first).
 template <typename T, int THREADS>
-__device__ __forceinline__ void fill_tile(const RowView<T>& in, const Slice<T, THREADS>& s, int tile, uint4* buf, uint64_t* bar) {
+__device__ __forceinline__ void fill_tile(const RowView<T>& in, const Slice<T, THREADS>& s, int tile, uint4* buf, uint64_t* bar, bool last) {
   const int b = s.begin(tile), e = s.end(tile);
   const int wb = max(b, in.whole_lo), we = min(e, in.whole_hi);
   if (threadIdx.x == 0) {
     const uint32_t bytes = we > wb ? (uint32_t)(we - wb) * 16u : 0u;
     const bool inside = LLMT_IN(in.at + wb * RowView<T>::N - in.off, in.at + max(we, wb) * RowView<T>::N - in.off, in.n, 601);
     sm100::bar_arrive_expect_tx(bar, inside ? bytes : 0u);
-    if (bytes && inside) sm100::bulk_load(buf + (wb - b), in.p + (wb * RowView<T>::N - in.off), bytes, bar);
+    if (bytes && inside) {
+      const T* src = in.p + (wb * RowView<T>::N - in.off);
+      if (last) sm100::bulk_load_once(buf + (wb - b), src, bytes, bar);
+      else sm100::bulk_load(buf + (wb - b), src, bytes, bar);
+    }
   }
   if (b < in.whole_lo && b < e && threadIdx.x == 0) buf[0] = load_part(in, b);
   if (e > in.whole_hi && e - 1 >= b && e - 1 >= in.whole_lo && threadIdx.x == (unsigned)((e - 1 - b) % THREADS))
@@ -329,7 +338,7 @@ __device__ __forceinline__ void store_pieces(const RowView<T>& out, const RowVie
 #pragma unroll 4
     for (int i = b + (int)threadIdx.x; i < we; i += THREADS) {
       const Piece<T> d = value(i);
-      if (i >= out.whole_lo) base[i] = make_uint4(d.u[0], d.u[1], d.u[2], d.u[3]);
+      if (i >= out.whole_lo) __stcs(base + i, make_uint4(d.u[0], d.u[1], d.u[2], d.u[3]));
     }
   }
   if (b < out.whole_lo && b < e && threadIdx.x == 0) store_part(out, like, b, value(b));
@@ -409,12 +418,12 @@ struct Tiles {
     }
   }
   __device__ __forceinline__ uint4* at(int tile) const { return buf + (tile & 1) * Slice<T, THREADS>::kTile; }
-  __device__ __forceinline__ void fill(int tile) const { fill_tile(in, s, tile, at(tile), &bar[tile & 1]); }
+  __device__ __forceinline__ void fill(int tile, bool last) const { fill_tile(in, s, tile, at(tile), &bar[tile & 1], last); }
   // Into the buffer of a tile that the CTA has read.
-  __device__ __forceinline__ void refill(int tile) const {
+  __device__ __forceinline__ void refill(int tile, bool last) const {
     __syncthreads();
     if (threadIdx.x == 0) sm100::fence_proxy_async_smem();
-    fill(tile);
+    fill(tile, last);
   }
   __device__ __forceinline__ const uint4* wait(int tile) {
     const int b = tile & 1;
@@ -459,8 +468,8 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(Toke
     const int tiles = s.tiles();
     Tiles<T, THREADS> held{in, s, buf, bar};
     held.init();
-    held.fill(0);  // thread 0 made the barriers
-    if (tiles > 1) held.fill(1);
+    held.fill(0, GRAD && tiles <= 2);  // thread 0 made the barriers
+    if (tiles > 1) held.fill(1, GRAD && tiles <= 3);
     // (a CTA's shared memory may be written by others once it has begun)
     if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     // what the token's loss needs, while the row is on its way
@@ -495,7 +504,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(Toke
       }
       ms.m = m;
       ms.s = sum.x + sum.y;
-      if (tile + 2 < tiles) held.refill(tile + 2);
+      if (tile + 2 < tiles) held.refill(tile + 2, GRAD && tile + 4 >= tiles);
     }
     ms.s = warp_sum(ms.s);
     // every warp's pair to every CTA of the cluster
@@ -540,7 +549,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(Toke
           const int first = s.begin(tile);
           store_pieces<T, THREADS>(out, in, first, s.end(tile),
                                    [&](int i) { return gradient_piece<T>(x[i - first], m, make_float2(k, k)); });
-          if (tile >= 2) held.refill(tile - 2);
+          if (tile >= 2) held.refill(tile - 2, true);
         }
         if (s.owns(((int)y + in.off) / Piece<T>::N)) gradient_target(out, (int)y, zy, m, k, c);
       }
@@ -584,8 +593,8 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) grad_rows_kernel(Token
   held.init();
   // the copies run while the slopes are waited for
   if (counts) {
-    held.fill(tiles - 1);
-    if (tiles > 1) held.fill(tiles - 2);
+    held.fill(tiles - 1, true);
+    if (tiles > 1) held.fill(tiles - 2, true);
   }
   pdl_wait();
   const float c = o.coef[n] * g;
@@ -604,7 +613,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) grad_rows_kernel(Token
     const int first = s.begin(tile);
     store_pieces<T, THREADS>(out, in, first, s.end(tile),
                              [&](int i) { return gradient_piece<T>(x[i - first], ms.x, make_float2(k, k)); });
-    if (tile >= 2) held.refill(tile - 2);
+    if (tile >= 2) held.refill(tile - 2, true);
   }
   if (mine) gradient_target(out, (int)y, zy, ms.x, k, c);
 }

@@ -233,6 +233,13 @@ std::vector<at::Tensor> rotary(at::Tensor q, c10::optional<at::Tensor> k, c10::o
   shape(q, "q");
   if (has_k) shape(*k, "k");
   CHECK(has_k || !k_out.has_value(), "rotary: k_out without k");
+  for (auto* y : {&q_out, &k_out})
+    if (y->has_value() && has_k && (*y)->numel() > 0 && k->numel() > 0 && q.numel() > 0) {
+      const void* other = y == &q_out ? k->data_ptr() : q.data_ptr();
+      CHECK((*y)->data_ptr() != other, "rotary: q_out is k, or k_out is q");
+    }
+  CHECK(!(q_out.has_value() && k_out.has_value() && q_out->numel() > 0 && q_out->data_ptr() == k_out->data_ptr()),
+        "rotary: q_out and k_out are the same values");
   llmt::RopeArgs a{};
   a.B = (int)B;
   a.T = (int)T;
@@ -349,6 +356,12 @@ struct MultiPlan {
       }
       t.push_back({static_cast<float*>(p[i].data_ptr()), g.data_ptr(), p16.empty() ? nullptr : p16[i].data_ptr(), numel[i],
                    (int32_t)first_block[i], 0, (float)wd[i], false});
+    }
+    if (zero_grad) {  // cleared by one tensor's blocks while another's read it
+      std::vector<const void*> at;
+      for (const auto& x : t) at.push_back(x.g);
+      std::sort(at.begin(), at.end());
+      CHECK(std::adjacent_find(at.begin(), at.end()) == at.end(), "adamw: zero_grad with one gradient for two tensors");
     }
     const int64_t n = 256 * blocks;
     const at::ScalarType dt_m = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat, dt_v = bits == 8 ? at::kByte : at::kFloat;
@@ -571,6 +584,7 @@ llmt::PolicyArgs policy_args(const c10::optional<at::Tensor>& old, const at::Ten
   no_grad_wanted(ref, "ref_logp");
   CHECK(clip_lo >= 0 && clip_lo <= 1 && clip_hi >= 0, "clip must be (low in [0, 1], high >= 0)");
   CHECK(reduction >= 0 && reduction <= 2, "unknown reduction");
+  CHECK(kl == 0 || (ref.has_value() && ref->defined()), "kl_coef without ref_logp");
   llmt::PolicyArgs q{};
   q.old = strided_bt<float>(old, at::kFloat, B, T, "old_logp");
   q.adv = strided_bt<float>(adv, at::kFloat, B, T, "advantages");
@@ -589,6 +603,7 @@ std::vector<at::Tensor> policy_rows(at::Tensor logits, at::Tensor targets, c10::
                                     bool keep) {
   llmt::TokenBatch a = logit_batch(logits, targets, mask);
   const llmt::PolicyArgs q = policy_args(old, adv, ref, a.B, a.T, clip_lo, clip_hi, kl, reduction);
+  CHECK(grad || !out.has_value(), "out without grad");
   llmt::RowOut o{};
   at::Tensor d, coef, stats;
   if (grad && out.has_value()) d = gradient_rows(logits, out, o);
@@ -662,6 +677,7 @@ std::vector<at::Tensor> preference_rows(at::Tensor logits, at::Tensor targets, c
                                         bool average, bool grad, c10::optional<at::Tensor> out, bool keep) {
   llmt::TokenBatch a = logit_batch(logits, targets, mask);
   const llmt::PreferenceArgs q = preference_args(ref, a.B, a.T, beta, smoothing, kind, average);
+  CHECK(grad || !out.has_value(), "out without grad");
   llmt::RowOut o{};
   at::Tensor d, coef, stats;
   if (grad && out.has_value()) d = gradient_rows(logits, out, o);

@@ -14,7 +14,7 @@ that counts has loss 0.
   preference_loss_tokens (llmt.models.native.NativeLlama.token_logprobs), behind autograd
 
 old_logp, ref_logp and advantages are constants of the loss (fp32; a tensor that requires a
-gradient is refused). Everything else about a loss is an argument of the call, and the kernels'
+gradient is refused), and a loss can be differentiated once. Everything else about a loss is an argument of the call, and the kernels'
 scratch is allocated per call, so calls on several streams or in several graphs share nothing.
 """
 from __future__ import annotations
@@ -22,6 +22,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from llmt.ops import native as N
 
@@ -126,6 +127,7 @@ class _PolicyRowsFn(torch.autograd.Function):
         return loss, logp
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g, _):
         logits, targets, mask, coef, stats = ctx.saved_tensors
         ready, ctx.ready = ctx.ready, None  # handed out once; a second backward makes its own
@@ -144,6 +146,7 @@ class _PreferenceRowsFn(torch.autograd.Function):
         return loss, logp, rewards
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g, _lp, _rw):
         logits, targets, mask, coef, stats = ctx.saved_tensors
         d = N.ext().grad_rows(logits.detach(), targets, mask, coef, stats, g.float().contiguous(), None, False)
@@ -172,6 +175,7 @@ class _PolicyTokensFn(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         (coef,) = ctx.saved_tensors
         return (coef * g,) + (None,) * 9
@@ -188,6 +192,7 @@ class _PreferenceTokensFn(torch.autograd.Function):
         return loss, rewards
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g, _):
         (coef,) = ctx.saved_tensors
         return (coef * g,) + (None,) * 8

@@ -20,6 +20,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from llmt.ops import native as N
 
@@ -110,7 +111,7 @@ class Rotary:
         fp16 / fp32 with unit stride along head_dim. positions: int32 or int64, (B, T) or (T,), None
         for 0 .. T - 1; a position outside (-2^31, 2^31) gives NaN. inverse turns back (with the
         scaling's factor, it is the gradient of the rotation). q_out / k_out take the results; they may be q and
-        k themselves. Returns new contiguous tensors otherwise."""
+        k themselves, and otherwise overlap no other operand. Returns new contiguous tensors otherwise."""
         if q.shape[-1] != self.head_dim:
             raise ValueError(f"head_dim of q is {q.shape[-1]}, of the plan {self.head_dim}")
         y, z = N.ext().rotary(q, k, positions, self.table, self.rotary_dim, self.interleaved, bool(inverse), q_out, k_out)
@@ -135,6 +136,7 @@ class _RotateBoth(torch.autograd.Function):
         return rot.rotate(q.detach(), k.detach(), positions)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         (positions,) = ctx.saved_tensors
         dq, dk = ctx.rot.rotate(_rows(dq), _rows(dk), positions, inverse=True)
@@ -149,6 +151,7 @@ class _RotateOne(torch.autograd.Function):
         return rot.rotate(q.detach(), None, positions)[0]
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq):
         (positions,) = ctx.saved_tensors
         return ctx.rot.rotate(_rows(dq), None, positions, inverse=True)[0], None, None

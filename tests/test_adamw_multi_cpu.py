@@ -36,6 +36,9 @@ def test_step_refusals():
     ]:
         with pytest.raises(RuntimeError, match=match):
             opt.step(g)
+    same = [torch.ones(4), torch.ones(4)]
+    with pytest.raises(RuntimeError, match="one gradient for two"):
+        MultiAdamW(same, zero_grad=True).step([same[0], same[0]])
     with pytest.raises(ValueError, match="dtype must be"):
         opt.state_values(torch.float16)
     assert MultiAdamW(p, state_bits=32).state_values()[0].dtype == torch.float32  # not decoded

@@ -29,6 +29,8 @@ def args(B=2, T=3, V=8):
     (lambda a: {"clip": (1.5, 0.2)}, "clip"),
     (lambda a: {"clip": (0.2, float("nan"))}, "clip"),
     (lambda a: {"out": torch.zeros(2, 3, 9)}, "out must match"),
+    (lambda a: {"out": a["logits"], "grad": False}, "out without grad"),
+    (lambda a: {"kl_coef": 0.1}, "kl_coef without"),
     (lambda a: {"out": torch.zeros(2, 3, 8, dtype=torch.half)}, "out must match"),
     (lambda a: {}, "CUDA tensor"),
 ])

@@ -72,7 +72,8 @@ def test_call_refusals():
         ((torch.zeros(2, 3, 4, 128)[..., ::2],), {}, "unit stride"),
         ((q, None, pos.float()), {}, "int32 or int64"), ((q, None, pos[:, :2]), {}, "positions must be"),
         ((q, None, pos[:, :1]), {}, "one position"), ((q, None, pos[None]), {}, "positions must be"),
-        ((q, None, pos), {"k_out": q}, "k_out without k"), ((q, None, pos), {}, "CUDA tensor"),
+        ((q, None, pos), {"k_out": q}, "k_out without k"),
+        ((q, q.clone(), pos), {"q_out": None, "k_out": q}, "k_out is q"), ((q, None, pos), {}, "CUDA tensor"),
     ]:
         with pytest.raises(RuntimeError, match=match):
             rot.rotate(*a, **kw)

@@ -203,6 +203,24 @@ __global__ void __launch_bounds__(256) count_tokens_kernel(TokenBatch a, int* co
   }
 }
 
+// Batches of at most this many tokens, averaged over tokens, are counted by each row's CTA while its row is on
+// the way, in place of a kernel before it (the call for 80 rows 16.2 -> 14.4 us of host time).
+constexpr int kCountHere = 512;
+__host__ __device__ inline bool counted_here(const TokenBatch& a, int reduction) {
+  return reduction == LOSS_SUM || (reduction == LOSS_TOKEN && (int64_t)a.B * a.T <= kCountHere);
+}
+__device__ __forceinline__ float token_weight_here(const TokenBatch& a, int reduction) {  // by one warp
+  if (reduction == LOSS_SUM) return 1.f;
+  const int n = a.B * a.T;
+  int sum = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x & 31; i < n; i += 32) {
+    int64_t y;
+    sum += token_counts(a, i / a.T, i % a.T, &y) ? 1 : 0;
+  }
+  return 1.f / (float)__reduce_add_sync(0xffffffffu, sum);
+}
+
 // Weight of a token of sequence b, by one warp (it sums the counts of all sequences).
 __device__ __forceinline__ float token_weight(const int* count, int B, int b, int reduction) {
   if (reduction == LOSS_SUM) return 1.f;
@@ -478,8 +496,12 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(Toke
     float weight = 0.f;
     if (POLICY && warp == 0) {
       token = load_token(q, b, t);
-      pdl_wait();  // the counts
-      weight = token_weight(o.count, a.B, b, q.reduction);
+      if (counted_here(a, q.reduction)) {
+        weight = token_weight_here(a, q.reduction);
+      } else {
+        pdl_wait();  // the counts
+        weight = token_weight(o.count, a.B, b, q.reduction);
+      }
     }
     MaxSum ms = {-INFINITY, 0.f};
     for (int tile = 0; tile < tiles; ++tile) {
@@ -563,7 +585,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(Toke
 __global__ void __launch_bounds__(1024) sum_rows_kernel(const float* x, int64_t n, float* out) {
   pdl_wait();
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 1024) s += (double)x[i];
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) s += (double)x[i];
   s = cta_sum(s);
   if (threadIdx.x == 0) *out = (float)s;
 }
@@ -634,27 +656,54 @@ __global__ void __launch_bounds__(kPairThreads) policy_tokens_kernel(TokenBatch 
   last_one_sums(o.ticket, 1, gridDim.x, o.loss_rows, (int64_t)a.B * a.T, 1.f, o.loss);
 }
 
-// One CTA per pair.
+// One CTA per pair, half of its threads for each sequence.
 __global__ void __launch_bounds__(kPairThreads) preference_kernel(TokenBatch a, PreferenceArgs q, const float* logp, RowOut o) {
+  constexpr int kHalf = kPairThreads / 2;
   const int p = blockIdx.x, P = gridDim.x;
+  const int side = threadIdx.x >= kHalf, own = p + side * P;
   pdl_trigger();
+  // what does not depend on the log-probabilities, of the first four tokens of each thread
+  bool counts[4];
+  float ref[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = (int)threadIdx.x % kHalf + i * kHalf;
+    int64_t y;
+    counts[i] = t < a.T && token_counts(a, own, t, &y);
+    ref[i] = counts[i] && q.ref.p ? q.ref.p[own * q.ref.sb + t * q.ref.st] : 0.f;
+  }
   pdl_wait();  // the log-probabilities
-  double gain[2];
-  int number[2];
-#pragma unroll 1
-  for (int side = 0; side < 2; ++side) {
-    const int b = p + side * P;
-    double s = 0.0;
-    int count = 0;
-    for (int t = threadIdx.x; t < a.T; t += blockDim.x) {
-      int64_t y;
-      if (!token_counts(a, b, t, &y)) continue;
-      s += (double)(logp[(int64_t)b * a.T + t] - (q.ref.p ? q.ref.p[b * q.ref.sb + t * q.ref.st] : 0.f));
-      ++count;
+  double s = 0.0;
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (counts[i]) {
+      s += (double)(logp[(int64_t)own * a.T + threadIdx.x % kHalf + i * kHalf] - ref[i]);
+      ++n;
     }
-    gain[side] = cta_sum(s);
-    number[side] = (int)cta_sum((double)count);
-    if (q.average) gain[side] /= (double)max(number[side], 1);
+  for (int t = (int)threadIdx.x % kHalf + 4 * kHalf; t < a.T; t += kHalf) {
+    int64_t y;
+    if (!token_counts(a, own, t, &y)) continue;
+    s += (double)(logp[(int64_t)own * a.T + t] - (q.ref.p ? q.ref.p[own * q.ref.sb + t * q.ref.st] : 0.f));
+    ++n;
+  }
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
+  n = __reduce_add_sync(0xffffffffu, n);
+  __shared__ double sums[kPairThreads / 32];
+  __shared__ int counted[kPairThreads / 32];
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s, counted[threadIdx.x >> 5] = n;
+  __syncthreads();
+  double gain[2] = {0.0, 0.0};
+  int number[2] = {0, 0};
+#pragma unroll
+  for (int w = 0; w < kPairThreads / 32; ++w) {
+    gain[w >= kHalf / 32] += sums[w];
+    number[w >= kHalf / 32] += counted[w];
+  }
+  if (q.average) {
+    gain[0] /= (double)max(number[0], 1);
+    gain[1] /= (double)max(number[1], 1);
   }
   const float D = (float)(gain[0] - gain[1]), x = q.beta * D;
   float loss, slope;  // of the pair, slope in D
@@ -670,15 +719,15 @@ __global__ void __launch_bounds__(kPairThreads) preference_kernel(TokenBatch a, 
     loss = off * off;
     slope = 2.f * off;
   }
-#pragma unroll 1
-  for (int side = 0; side < 2; ++side) {
-    const int b = p + side * P;
-    const float c = (side ? -slope : slope) / (float)P / (q.average ? (float)max(number[side], 1) : 1.f);
-    for (int t = threadIdx.x; t < a.T; t += blockDim.x) {
-      int64_t y;
-      o.coef[(int64_t)b * a.T + t] = token_counts(a, b, t, &y) ? c : 0.f;
-    }
-    if (threadIdx.x == 0) o.rewards[b] = (float)((double)q.beta * gain[side]);
+  const float c = (side ? -slope : slope) / (float)P / (q.average ? (float)max(side ? number[1] : number[0], 1) : 1.f);
+  for (int t = (int)threadIdx.x % kHalf; t < a.T; t += kHalf) {
+    int64_t y;
+    o.coef[(int64_t)own * a.T + t] = token_counts(a, own, t, &y) ? c : 0.f;
+  }
+  if (threadIdx.x % kHalf == 0) o.rewards[own] = (float)((double)q.beta * (side ? gain[1] : gain[0]));
+  if (P == 1) {
+    if (threadIdx.x == 0) *o.loss = loss;
+    return;
   }
   if (threadIdx.x == 0) o.loss_rows[p] = loss;
   last_one_sums(o.ticket, 1, P, o.loss_rows, P, 1.f / (float)P, o.loss);
@@ -728,19 +777,19 @@ cudaError_t launch_rows(const TokenBatch& a, RowShape r, bool pdl, cudaStream_t 
 }
 
 template <typename T, bool POLICY, bool GRAD>
-cudaError_t rows_of(const TokenBatch& a, RowShape r, const PolicyArgs& q, const RowOut& o, cudaStream_t st) {
+cudaError_t rows_of(const TokenBatch& a, RowShape r, const PolicyArgs& q, const RowOut& o, bool pdl, cudaStream_t st) {
   switch (r.threads) {
-    case 128: return launch_rows<token_rows_kernel<T, 128, POLICY, GRAD>>(a, r, POLICY, st, a, q, o, r.ctas);
-    default: return launch_rows<token_rows_kernel<T, 256, POLICY, GRAD>>(a, r, POLICY, st, a, q, o, r.ctas);
+    case 128: return launch_rows<token_rows_kernel<T, 128, POLICY, GRAD>>(a, r, pdl, st, a, q, o, r.ctas);
+    default: return launch_rows<token_rows_kernel<T, 256, POLICY, GRAD>>(a, r, pdl, st, a, q, o, r.ctas);
   }
 }
 template <bool POLICY, bool GRAD>
-cudaError_t rows(const TokenBatch& a, const PolicyArgs& q, const RowOut& o, cudaStream_t st) {
+cudaError_t rows(const TokenBatch& a, const PolicyArgs& q, const RowOut& o, bool pdl, cudaStream_t st) {
   const RowShape r = row_shape(a);
   switch (a.dtype) {
-    case 0: return rows_of<bf16, POLICY, GRAD>(a, r, q, o, st);
-    case 1: return rows_of<__half, POLICY, GRAD>(a, r, q, o, st);
-    default: return rows_of<float, POLICY, GRAD>(a, r, q, o, st);
+    case 0: return rows_of<bf16, POLICY, GRAD>(a, r, q, o, pdl, st);
+    case 1: return rows_of<__half, POLICY, GRAD>(a, r, q, o, pdl, st);
+    default: return rows_of<float, POLICY, GRAD>(a, r, q, o, pdl, st);
   }
 }
 template <typename T>
@@ -762,15 +811,19 @@ cudaError_t check(const TokenBatch& a) {
 
 cudaError_t logprob_rows(const TokenBatch& a, const RowOut& o, cudaStream_t st) {
   if (cudaError_t e = check(a)) return e;
-  return rows<false, false>(a, PolicyArgs{}, o, st);
+  return rows<false, false>(a, PolicyArgs{}, o, false, st);
 }
 
 cudaError_t policy_rows(const TokenBatch& a, const PolicyArgs& q, const RowOut& o, cudaStream_t st) {
   if (cudaError_t e = check(a)) return e;
-  count_tokens_kernel<<<a.B, 256, 0, st>>>(a, o.count, o.ticket);
-  if (cudaError_t e = cudaGetLastError()) return e;
-  if (cudaError_t e = o.dz ? rows<true, true>(a, q, o, st) : rows<true, false>(a, q, o, st)) return e;
-  return launch_pdl_if(true, sum_rows_kernel, 1, 1024, 0, st, (const float*)o.loss_rows, (int64_t)a.B * a.T, o.loss);
+  const bool count = !counted_here(a, q.reduction);
+  if (count) {
+    count_tokens_kernel<<<a.B, 256, 0, st>>>(a, o.count, o.ticket);
+    if (cudaError_t e = cudaGetLastError()) return e;
+  }
+  if (cudaError_t e = o.dz ? rows<true, true>(a, q, o, count, st) : rows<true, false>(a, q, o, count, st)) return e;
+  const int64_t n = (int64_t)a.B * a.T;
+  return launch_pdl_if(true, sum_rows_kernel, 1, n <= 2048 ? 128 : 1024, 0, st, (const float*)o.loss_rows, n, o.loss);
 }
 
 cudaError_t policy_tokens(const TokenBatch& a, const PolicyArgs& q, const float* logp, const RowOut& o, cudaStream_t st) {

@@ -68,12 +68,12 @@ def _clip(clip):
 def logprob_rows(logits, targets, mask=None):
     """(B, T) fp32 log-probabilities of the targets under logits (B, T, V) bf16 / fp16 / fp32; 0 where
     a token does not count. No gradient: see policy_loss, preference_loss and token_logprobs."""
-    return N.ext().logprob_rows(logits.detach(), targets, mask)[0]
+    return N.ext().logprob_rows(logits, targets, mask)[0]
 
 
 def _policy_rows(logits, targets, old_logp, advantages, ref_logp, mask, clip, kl_coef, reduction, grad, out=None, keep=False):
     lo, hi = _clip(clip)
-    return N.ext().policy_rows(logits.detach(), targets, old_logp, advantages, ref_logp, mask, lo, hi, float(kl_coef),
+    return N.ext().policy_rows(logits, targets, old_logp, advantages, ref_logp, mask, lo, hi, float(kl_coef),
                                _choice(REDUCTIONS, reduction, "reduction"), bool(grad), out, keep)
 
 
@@ -105,7 +105,7 @@ def preference_loss_rows(logits, targets, ref_logp=None, mask=None, beta=0.1, ki
         ipo:     (D - 1 / (2 beta))^2
     averaged over pairs. Returns PreferenceRows(loss, logp, rewards = beta * gains (2 P), dlogits)."""
     loss, logp, rewards, d, _, _ = N.ext().preference_rows(
-        logits.detach(), targets, ref_logp, mask, float(beta), float(label_smoothing), _choice(KINDS, kind, "kind"), bool(average),
+        logits, targets, ref_logp, mask, float(beta), float(label_smoothing), _choice(KINDS, kind, "kind"), bool(average),
         bool(grad), out)
     return PreferenceRows(loss, logp, rewards, d if grad else None)
 
@@ -131,7 +131,7 @@ class _PolicyRowsFn(torch.autograd.Function):
     def backward(ctx, g, _):
         logits, targets, mask, coef, stats = ctx.saved_tensors
         ready, ctx.ready = ctx.ready, None  # handed out once; a second backward makes its own
-        d = N.ext().grad_rows(logits.detach(), targets, mask, coef, stats, g.float().contiguous(), ready, ready is not None)
+        d = N.ext().grad_rows(logits, targets, mask, coef, stats, g.float().contiguous(), ready, ready is not None)
         return (d,) + (None,) * 8
 
 
@@ -139,7 +139,7 @@ class _PreferenceRowsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, ref_logp, mask, beta, kind, label_smoothing, average):
         loss, logp, rewards, _, coef, stats = N.ext().preference_rows(
-            logits.detach(), targets, ref_logp, mask, float(beta), float(label_smoothing), _choice(KINDS, kind, "kind"),
+            logits, targets, ref_logp, mask, float(beta), float(label_smoothing), _choice(KINDS, kind, "kind"),
             bool(average), False, None, True)
         ctx.save_for_backward(logits, targets, mask, coef, stats)
         ctx.mark_non_differentiable(logp, rewards)
@@ -149,7 +149,7 @@ class _PreferenceRowsFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g, _lp, _rw):
         logits, targets, mask, coef, stats = ctx.saved_tensors
-        d = N.ext().grad_rows(logits.detach(), targets, mask, coef, stats, g.float().contiguous(), None, False)
+        d = N.ext().grad_rows(logits, targets, mask, coef, stats, g.float().contiguous(), None, False)
         return (d,) + (None,) * 7
 
 

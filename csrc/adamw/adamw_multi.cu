@@ -52,8 +52,7 @@ __device__ __forceinline__ uint32_t scale_byte_v(uint32_t top) { return scale_by
 // Both codes are bits 20 to 27 of an fp32 number: scaled so that the format's subnormals are fp32's
 // subnormals, adding 20 random bits below the kept ones and cutting rounds up with the right
 // probability, in the normal and the subnormal range alike. Here they are shifted to the top byte, where
-// four of them are gathered by byte permutations, as the noise is made: the kernel is bound by its
-// integer instructions. noise: bits 8 to 23 random, bit 7 set (half a last step). A block's scale keeps
+// four of them are gathered by byte permutations, as the noise is made. noise: bits 8 to 23 random, bit 7 set (half a last step). A block's scale keeps
 // every finite value within the format; infinities and NaN are put right afterwards (code_of_bad_*).
 __device__ __forceinline__ uint32_t encode_m(float m, float unscale, uint32_t noise) {  // without the sign
   return (__float_as_uint(__fmul_rn(__fmul_rn(fabsf(m), unscale), 0x1p-120f)) << 4) + noise;
@@ -330,8 +329,8 @@ __device__ __forceinline__ int find_tensor(const Batch<CAP>& batch, int64_t w, i
 }
 
 // Bound by memory with 32-bit states: 24 to 28 bytes a value, 103% of the measured copy rate for 0.94G values
-// (3.90 ms). With 8-bit states, 16 to 18 bytes, by instructions too: 72% of the issue slots at 87% of that rate
-// (375M values 1.19 ms). A CTA takes a run of `rounds` blocks a warp, consecutive warps consecutive blocks,
+// (3.90 ms). With 8-bit states, 16 to 18 bytes, it uses 72% of the issue slots at about 87% of that rate
+// (375M values 1.19 ms); 11% fewer instructions, or two blocks a warp at once, were no faster. A CTA takes a run of `rounds` blocks a warp, consecutive warps consecutive blocks,
 // and ends: the memory serves a few hundred short runs, handed out in order, at its copy rate, but a
 // persistent grid that sweeps through all tensors together at 88% (4.57 ms), and one whose CTAs step
 // through runs of their own at 85%. Blocks brought to shared memory by asynchronous copies one ahead

@@ -2,8 +2,8 @@
 preference loss over pairs of sequences, on logits (B, T, V) or on log-probabilities (B, T).
 
 A token counts where its mask is set (every token without a mask) and its target is an id of the
-vocabulary; the logits of the others are not read and get a zero gradient. A batch without a token
-that counts has loss 0.
+vocabulary; the logits of the others are not read and get a zero gradient. Without a token that
+counts a policy loss is 0 and a sequence's gain is 0.
 
   logprob_rows           log-probabilities of the targets
   policy_loss_rows       loss, log-probabilities and the gradient of the logits in one call: the
@@ -14,8 +14,9 @@ that counts has loss 0.
   preference_loss_tokens (llmt.models.native.NativeLlama.token_logprobs), behind autograd
 
 old_logp, ref_logp and advantages are constants of the loss (fp32; a tensor that requires a
-gradient is refused), and a loss can be differentiated once. Everything else about a loss is an argument of the call, and the kernels'
-scratch is allocated per call, so calls on several streams or in several graphs share nothing.
+gradient is refused), and a loss can be differentiated once. Everything else about a loss is an
+argument of the call, and the kernels' scratch is allocated per call, so calls on several streams
+or in several graphs share nothing.
 """
 from __future__ import annotations
 

@@ -56,6 +56,7 @@ class _Counted:
         def call(*a, **kw):
             LAUNCHES.count += k
             return fn(*a, **kw)
+        self.__dict__[name] = call  # made once: the next access does not come here
         return call
 
 

@@ -248,7 +248,7 @@ __device__ __forceinline__ void whole_block(const MultiTensor& t, const MultiHyp
 // Starts bringing a block into L2: one 128-byte line a lane. With 8-bit states the warps' own loads (registers
 // for one block each) are not enough bytes in flight: with the next block asked for under the present one's
 // arithmetic they wait for L2 instead of memory (2.39 -> 1.85 ms in runs of 8). With 32-bit states they are
-// enough, and asking ahead costs 4%.
+// enough.
 template <typename G, int BITS>
 __device__ __forceinline__ void prefetch_block(const MultiTensor& t, const MultiState& s, int64_t at, int64_t blk, int lane) {
   constexpr int kStateLine = BITS == 32 ? 32 : 128;  // values in a line
@@ -328,13 +328,13 @@ __device__ __forceinline__ int find_tensor(const Batch<CAP>& batch, int64_t w, i
   return at + __popc(__ballot_sync(0xffffffffu, lane < step && i < batch.count && batch.t[min(i, CAP - 1)].first_work <= w)) - 1;
 }
 
-// Bound by memory with 32-bit states: 24 to 28 bytes a value, 103% of the measured copy rate for 0.94G values
-// (3.90 ms). With 8-bit states, 16 to 18 bytes, it uses 72% of the issue slots at about 87% of that rate
-// (375M values 1.19 ms); 11% fewer instructions, or two blocks a warp at once, were no faster. A CTA takes a run of `rounds` blocks a warp, consecutive warps consecutive blocks,
-// and ends: the memory serves a few hundred short runs, handed out in order, at its copy rate, but a
-// persistent grid that sweeps through all tensors together at 88% (4.57 ms), and one whose CTAs step
-// through runs of their own at 85%. Blocks brought to shared memory by asynchronous copies one ahead
-// were slower with 8 bits (1.95 ms against 1.80, moments decoded) and no faster with 32.
+// Bound by memory: with 32-bit states 28 to 30 bytes a value, 103% of the measured copy rate for 0.94G values
+// (3.90 ms); with 8-bit states 16 to 18 bytes, 97% for 374M values (1.06 ms), at 72% of the issue slots.
+// A CTA takes a run of `rounds` blocks a warp, consecutive warps consecutive blocks, and ends: the memory
+// serves a few hundred short runs, handed out in order, at its copy rate, but a persistent grid at 88%
+// (4.57 ms), whether it sweeps through all tensors together or each CTA steps through runs of its own.
+// Blocks brought to shared memory by asynchronous copies one ahead were slower with 8 bits (1.95 ms
+// against 1.80, moments decoded) and no faster with 32.
 template <typename G, int BITS, int CAP>
 __global__ void __launch_bounds__(kThreads, 4) adamw_multi_kernel(const __grid_constant__ Batch<CAP> batch, MultiHyper h,
                                                                   MultiState s, int blocks, int rounds, bool last_launch) {
@@ -433,7 +433,7 @@ cudaError_t launch(const MultiTensor* t, int count, const MultiHyper& h, const M
   b.count = count;
   LLMT_REQUIRE(blocks < 0x7fffffff, "adamw_multi: too many values for one launch");
   // whole waves of CTAs of at most `most` rounds. 8-bit blocks are small beside a CTA's start, in which the
-  // arguments and the step's constants are waited for: 375M values with moments decoded take 1.88 ms in
+  // arguments and the step's constants are waited for: 375M values with moments decoded take 1.85 ms in
   // runs of 8, 1.65 of 16, 1.61 of 32; 0.94G 32-bit values 3.90 ms in runs of 4, 3.97 of 8, 4.03 of 16
   constexpr int64_t most = BITS == 8 ? 32 : 4;
   const int64_t slots = (int64_t)sm_count() * 4 * (kThreads / 32), waves = cdiv(blocks, slots * most);

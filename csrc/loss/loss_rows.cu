@@ -580,8 +580,8 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(Toke
 }
 
 // The loss from its rows, in a fixed order. A kernel of its own: a ticket taken by each row's CTA needs a
-// fence after the row's loss, and the fence waits for the CTA's gradient to reach memory (18 us of 120
-// at 4096 rows of 32000 bf16).
+// fence after the row's loss, and the fence waits for the CTA's gradient to reach memory (10 us of
+// 110 at 4096 rows of 32000 bf16).
 __global__ void __launch_bounds__(1024) sum_rows_kernel(const float* x, int64_t n, float* out) {
   pdl_wait();
   double s = 0.0;

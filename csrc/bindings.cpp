@@ -365,10 +365,15 @@ struct MultiPlan {
                    (int32_t)first_block[i], 0, (float)wd[i], false});
     }
     if (zero_grad) {  // cleared by one tensor's blocks while another's read it
-      std::vector<const void*> at;
-      for (const auto& x : t) at.push_back(x.g);
-      std::sort(at.begin(), at.end());
-      CHECK(std::adjacent_find(at.begin(), at.end()) == at.end(), "adamw: zero_grad with one gradient for two tensors");
+      std::vector<std::pair<const char*, const char*>> spans;
+      spans.reserve(t.size());
+      for (const auto& x : t) {
+        const char* g = static_cast<const char*>(x.g);
+        spans.emplace_back(g, g + (bf16 ? 2 : 4) * x.n);
+      }
+      std::sort(spans.begin(), spans.end());
+      for (size_t i = 1; i < spans.size(); ++i)
+        CHECK(spans[i].first >= spans[i - 1].second, "adamw: zero_grad with one gradient for two tensors");
     }
     const int64_t n = 256 * blocks;
     const at::ScalarType dt_m = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat, dt_v = bits == 8 ? at::kByte : at::kFloat;

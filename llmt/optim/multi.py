@@ -61,7 +61,8 @@ class MultiAdamW:
     @torch.no_grad()
     def step(self, grads=None):
         """One step on `grads` (one per tensor, all fp32 or all bf16; None leaves a tensor and its states
-        as they are) or on the buffers given at construction."""
+        as they are) or on the buffers given at construction. The step count, and with it the bias
+        correction, is one for all tensors, those left out included. With zero_grad the gradients may not overlap."""
         grads = self.grads if grads is None else grads
         if grads is None:
             raise ValueError("no gradients: give them to step() or to MultiAdamW")

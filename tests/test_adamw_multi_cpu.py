@@ -44,6 +44,14 @@ def test_step_refusals():
     assert MultiAdamW(p, state_bits=32).state_values()[0].dtype == torch.float32  # not decoded
 
 
+def test_gradients_that_overlap_in_part_are_not_cleared():
+    p, g = [torch.zeros(4), torch.zeros(4)], torch.ones(9)
+    with pytest.raises(RuntimeError, match="one gradient for two"):
+        MultiAdamW(p, zero_grad=True).step([g[2:6], g[5:9]])
+    with pytest.raises(RuntimeError, match="CUDA tensor"):  # side by side: refused for the device alone
+        MultiAdamW(p, zero_grad=True).step([g[4:8], g[:4]])
+
+
 def test_layout():
     opt = MultiAdamW([torch.zeros(1), torch.zeros(256), torch.zeros(257), torch.zeros(3)])
     assert opt.plan.blocks == 5 and list(opt.plan.first_block) == [0, 1, 2, 4]

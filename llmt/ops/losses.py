@@ -157,6 +157,8 @@ class _PreferenceRowsFn(torch.autograd.Function):
 def policy_loss(logits, targets, old_logp, advantages, ref_logp=None, mask=None, clip=(0.2, 0.2), kl_coef=0.0,
                 reduction="token"):
     """policy_loss_rows behind autograd: PolicyLoss(loss, logp); loss.backward() reaches the logits."""
+    if not torch.is_grad_enabled():
+        logits = logits.detach()  # a Function is told of the logits' flag alone: it would write their gradient
     return PolicyLoss(*_PolicyRowsFn.apply(logits, targets, old_logp, advantages, ref_logp, mask, clip, kl_coef, reduction))
 
 

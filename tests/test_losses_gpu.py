@@ -274,6 +274,20 @@ def test_autograd(L, scale):
     assert ((leaf.grad.double() - rows.dlogits.double() * scale).abs() <= 2.1 * u * rows.dlogits.double().abs() * scale).all()
 
 
+def test_no_grad_writes_no_gradient(L):
+    z, y, m, old, ref, adv = make(2, 64, 8192, "fp32")
+    z.requires_grad_()
+    want = L.policy_loss(z, y, old, adv, ref, m, kl_coef=0.1)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        got = L.policy_loss(z, y, old, adv, ref, m, kl_coef=0.1)
+    assert torch.cuda.max_memory_allocated() - before < z.numel()  # a gradient is 4 bytes a value
+    assert not got.loss.requires_grad
+    assert ((got.logp - want.logp).abs() <= 2 ** -14 + 2 ** -21 * want.logp.abs()).all()  # each is off by half of that
+
+
 def test_token_forms_match_rows(L):
     z, y, m, old, ref, adv = make(4, 9, 2000, "fp32")
     leaf = L.logprob_rows(z, y, m).requires_grad_()

@@ -16,7 +16,9 @@ counts a policy loss is 0 and a sequence's gain is 0.
 old_logp, ref_logp and advantages are constants of the loss (fp32; a tensor that requires a
 gradient is refused), and a loss can be differentiated once. Everything else about a loss is an
 argument of the call, and the kernels' scratch is allocated per call, so calls on several streams
-or in several graphs share nothing.
+or in several graphs share nothing. To capture a backward pass into a CUDA graph, drop the results of
+eager calls on the same leaves first: autograd adds a leaf's gradient on the stream of the oldest
+graph that still holds it, which a capture on another stream does not allow.
 """
 from __future__ import annotations
 

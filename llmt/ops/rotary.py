@@ -119,7 +119,8 @@ class Rotary:
         return y, (z if k is not None else None)
 
     def apply(self, q, k=None, positions=None):
-        """rotate behind autograd; the backward is one inverse rotation of both gradients."""
+        """rotate behind autograd; the backward is one inverse rotation of both gradients. Before it is
+        captured into a CUDA graph, drop the results of eager calls on the same leaves."""
         if k is None:
             return _RotateOne.apply(q, positions, self), None
         return _RotateBoth.apply(q, k, positions, self)

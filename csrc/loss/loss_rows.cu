@@ -434,6 +434,7 @@ struct Tiles {
       sm100::fence_barrier_init();
       sm100::fence_proxy_async_smem();
     }
+    __syncwarp();  // the other lanes of the warp that polls come to the barriers after they are made
   }
   __device__ __forceinline__ uint4* at(int tile) const { return buf + (tile & 1) * Slice<T, THREADS>::kTile; }
   __device__ __forceinline__ void fill(int tile, bool last) const { fill_tile(in, s, tile, at(tile), &bar[tile & 1], last); }

@@ -252,10 +252,13 @@ __device__ __forceinline__ PolicyToken load_token(const PolicyArgs& q, int b, in
 __device__ __forceinline__ void policy_token(const PolicyArgs& q, PolicyToken k, float logp, float w, float* loss,
                                              float* slope) {
   const float A = k.adv, r = q.old.p ? expf(logp - k.old) : (logp == logp ? 1.f : logp);
-  const float free = r * A, held = fminf(fmaxf(r, 1.f - q.clip_lo), 1.f + q.clip_hi) * A;
-  // written so that a NaN ratio or advantage stays one (fminf and fmaxf drop it)
-  float l = r != r ? r : -(free <= held ? free : held);
-  float c = free <= held || r != r ? -free : 0.f;
+  // an advantage of zero takes no part, a ratio past fp32 included (inf * 0 would be NaN)
+  const float free = A == 0.f ? 0.f : r * A;
+  const float held = A == 0.f ? 0.f : fminf(fmaxf(r, 1.f - q.clip_lo), 1.f + q.clip_hi) * A;
+  // a NaN ratio or advantage stays one in the loss and in the slope: fminf, fmaxf and comparisons drop it
+  const bool bad = r != r || A != A;
+  float l = bad ? NAN : -(free <= held ? free : held);
+  float c = bad ? NAN : free <= held ? -free : 0.f;
   if (q.ref.p) {
     const float d = k.ref - logp;
     const float e = expm1f(d);  // e^d - 1 - d without losing a small d

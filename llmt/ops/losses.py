@@ -89,7 +89,8 @@ def policy_loss_rows(logits, targets, old_logp, advantages, ref_logp=None, mask=
     averaged over the tokens that count ("token"), over sequences of their own averages
     ("sequence", sequences without such tokens left out), or summed ("sum").
     old_logp None takes the current log-probabilities (the first step on a batch); advantages are
-    (B, T) or broadcast to it, (B, 1) for one per sequence. `out` takes the gradient; it may be the
+    (B, T) or broadcast to it, (B, 1) for one per sequence; one of zero takes no part whatever the
+    ratio, a NaN makes the loss and its own row of the gradient NaN. `out` takes the gradient; it may be the
     logits themselves. Returns PolicyRows(loss, logp, dlogits)."""
     loss, logp, d, _, _ = _policy_rows(logits, targets, old_logp, advantages, ref_logp, mask, clip, kl_coef, reduction,
                                        grad, out)

@@ -373,14 +373,12 @@ __device__ __forceinline__ void zero_row(const RowView<T>& out, int rank, int ct
   store_pieces<T, THREADS>(out, out, s.lo, s.hi, [](int) { return Piece<T>{{0u, 0u, 0u, 0u}}; });
 }
 
-// One tile of the gradient without the target's own term: k e^(z - M). For the 16-bit types the exponent
-// is one fused multiply-add, z log2(e) - M log2(e), off by 2^-24 of M log2(e); fp32 subtracts first.
-template <typename T>
+// Two values of the gradient without the target's own term: k e^(z - M). The maximum is subtracted first, for
+// every type: a multiply-add of z around a rounded M log2(e) would be off by 2^-24 of M log2(e) (1.3e-3 of the
+// gradient at fp16 logits of 6e4, most of it at bf16 ones of 1e8), and at the maximum itself by enough to turn the
+// sign of c (1 - p) of a token that is almost certain.
 __device__ __forceinline__ float2 gradient_pair(float2 z, float m, float2 k2) {
-  const float2 l2 = make_float2(kLog2e, kLog2e);
-  float2 t;
-  if constexpr (sizeof(T) == 4) t = sm100::mul2(sm100::add2(z, make_float2(-m, -m)), l2);
-  else t = sm100::fma2(z, l2, make_float2(-m * kLog2e, -m * kLog2e));
+  const float2 t = sm100::mul2(sm100::add2(z, make_float2(-m, -m)), make_float2(kLog2e, kLog2e));
   return sm100::mul2(k2, make_float2(sm100::ex2_approx(t.x), sm100::ex2_approx(t.y)));
 }
 template <typename T>
@@ -388,13 +386,13 @@ __device__ __forceinline__ Piece<T> gradient_piece(uint4 v, float m, float2 k2) 
   const Piece<T> x = {{v.x, v.y, v.z, v.w}};
   Piece<T> d;
 #pragma unroll
-  for (int h = 0; h < Piece<T>::N / 2; ++h) put_pair(d, h, gradient_pair<T>(pair_of(x, h), m, k2));
+  for (int h = 0; h < Piece<T>::N / 2; ++h) put_pair(d, h, gradient_pair(pair_of(x, h), m, k2));
   return d;
 }
 // The target's value once more, with its own term, by the thread that stored its piece.
 template <typename T>
 __device__ __forceinline__ void gradient_target(const RowView<T>& out, int y, float zy, float m, float k, float c) {
-  out.p[y] = from_f<T>(gradient_pair<T>(make_float2(zy, zy), m, make_float2(k, k)).x + c);
+  out.p[y] = from_f<T>(gradient_pair(make_float2(zy, zy), m, make_float2(k, k)).x + c);
 }
 
 // Maximum and sum of the whole row from those of each warp, by one warp; a row with an infinite or NaN

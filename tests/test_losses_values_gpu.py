@@ -32,3 +32,41 @@ def test_an_advantage_of_zero_takes_no_part(L, clip):  # noqa: F811
     adv[0, 1], old[0, 1] = 0.0, -200.0
     r = L.policy_loss_rows(z, y, old, adv, clip=clip, reduction="sum")
     assert r.loss.isfinite() and (r.dlogits[0, 1] == 0).all() and r.dlogits.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype,offset", [("bf16", 100.0), ("bf16", 1e3), ("bf16", 1e6), ("bf16", -1e30), ("fp16", 2e3),
+                                          ("fp16", 6e4), ("fp32", 1e4)])
+@pytest.mark.parametrize("V", [50, 40000])
+def test_a_common_offset_leaves_the_gradient(L, dtype, offset, V):  # noqa: F811
+    """softmax(z + a) = softmax(z): the exponents are differences of logits, as exact as those are (the other tests' bounds)."""
+    z, y, m, _, _, adv = make(2, 3, V, dtype, seed=V)
+    z = (z.float() + offset).to(z.dtype)
+    c = counted(z, y, m)
+    lp = oracle_logp(z, y, c)
+    _, slope, terms = policy_oracle(lp, c, None, adv, None, (0.2, 0.2), 0.0, "sum")
+    r = L.policy_loss_rows(z, y, None, adv, mask=m, reduction="sum")
+    check_gradient(r.dlogits, z, y, c, slope, 2.0 ** -14 * terms)
+    leaf = z.clone().requires_grad_()
+    (L.policy_loss(leaf, y, None, adv, mask=m, reduction="sum").loss * 0.5).backward()
+    check_gradient(leaf.grad, z, y, c, slope * 0.5, 2.0 ** -15 * terms)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("drop", [18.0, 23.0])
+def test_gradient_of_an_almost_certain_token(L, dtype, drop):  # noqa: F811
+    """The target's own gradient c (1 - p) for 1 - p = 999 e^-drop (1.5e-5, 1e-7) and maxima of 8 to 120. The sum 1 + t of the
+    row is at least 1 after any rounding, so the sign is c's or the value zero; it is off by at most 16
+    additions' half steps of 2^-24 (a thread's, five steps of its warp, the warps' join) and c / s by one more."""
+    T = 225
+    top = 8.0 + 0.5 * torch.arange(T, device="cuda")
+    z = (top - drop)[None, :, None].expand(1, T, 1000).contiguous().to({"bf16": torch.bfloat16, "fp16": torch.float16}.get(dtype, torch.float32))
+    y = torch.arange(T, device="cuda")[None] * 4
+    z.scatter_(-1, y[..., None], top.to(z.dtype)[None, :, None])
+    adv = torch.ones(1, T, device="cuda")
+    d = L.policy_loss_rows(z, y, None, adv, reduction="sum").dlogits
+    got = -d.gather(-1, y[..., None]).double()
+    want = 1 - torch.softmax(z.double(), -1).gather(-1, y[..., None])
+    assert (got >= 0).all(), got.min().item()
+    u = torch.finfo(z.dtype).eps / 2
+    tiny = 2.0 ** -25 if dtype == "fp16" else 0.0
+    assert ((got - want).abs() <= 17 * 2.0 ** -24 + u * want + tiny).all()

@@ -43,21 +43,14 @@ constexpr int kFill = 4;                // CTAs a SM up to which few rows are sp
 constexpr int kPairThreads = 256;
 
 // Exponentials. Errors of one sign matter here: those of 700 tokens' log-probabilities add up in the
-// reward of their sequence. log2(e) in one fp32 number is 1.3e-8 short, which makes an e^-8 1e-7 too large:
-// it has a second part below. The exponential of two is up to 8e-7 off and 5e-8 short in the mean
+// reward of their sequence. log2(e) in one fp32 number is 1.3e-8 short, which makes an e^-8 1e-7 too large: it is
+// held in two parts, the second what the first leaves (a product with a constant to more than its type's digits:
+// Dekker, Numerische Mathematik 18, 1971). The exponential of two is up to 8e-7 off and 5e-8 short in the mean
 // (measured on 2^20 arguments each in [-4 k - 4, -4 k], k = 0 .. 4: 4.5e-8 to 5.1e-8), which a row's
-// logarithm takes back (kShort); splitting the integer off first, as exp_ does for the few terms that join
-// sums, leaves 1e-8 but takes three more instructions a value (of 4.4 here).
-constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596299e-8f;
+// logarithm takes back (kShort). The few factors that join a row's sums are expf.
+constexpr double kLog2eExact = 1.4426950408889634074;
+constexpr float kLog2e = (float)kLog2eExact, kLog2eLow = (float)(kLog2eExact - (double)kLog2e);
 constexpr double kShort = 5e-8;
-// e^x for x <= 0; e^-87 below that.
-__device__ __forceinline__ float exp_(float x) {
-  x = fmaxf(x, -87.f);
-  const float magic = 12582912.f;  // 1.5 2^23: adding it leaves the integer in the low bits
-  const float t = fmaf(x, kLog2e, magic);
-  const float f = fmaf(x, kLog2eLow, fmaf(x, kLog2e, magic - t));
-  return __uint_as_float(__float_as_uint(sm100::ex2_approx(f)) + (__float_as_uint(t) << 23));
-}
 // sum + e^(z - at), two values at a time.
 __device__ __forceinline__ float2 add_exp(float2 z, float2 minus_at, float2 sum) {
   const float2 x = sm100::add2(z, minus_at);
@@ -402,7 +395,7 @@ __device__ __forceinline__ MaxSum join_warps(const MaxSum* part, int n) {
   for (int i = threadIdx.x & 31; i < n; i += 32) m = max_nan(m, part[i].m);
 #pragma unroll
   for (int w = 16; w > 0; w >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, w));
-  for (int i = threadIdx.x & 31; i < n; i += 32) s += part[i].s * exp_(part[i].m - m);
+  for (int i = threadIdx.x & 31; i < n; i += 32) s += part[i].s * expf(part[i].m - m);
   s = warp_sum(s);
   if (!(fabsf(m) < INFINITY)) s = NAN;
   return {m, s};
@@ -518,7 +511,7 @@ __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(Toke
 #pragma unroll
       for (int w = 16; w > 0; w >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, w));
       const float at = m == -INFINITY ? 0.f : m;
-      float2 sum = make_float2(ms.s == 0.f ? 0.f : ms.s * exp_(ms.m - at), 0.f);
+      float2 sum = make_float2(ms.s == 0.f ? 0.f : ms.s * expf(ms.m - at), 0.f);
 #pragma unroll 4
       for (int i = threadIdx.x; i < count; i += THREADS) {
         const uint4 v = x[i];

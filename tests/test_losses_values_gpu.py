@@ -70,3 +70,15 @@ def test_gradient_of_an_almost_certain_token(L, dtype, drop):  # noqa: F811
     u = torch.finfo(z.dtype).eps / 2
     tiny = 2.0 ** -25 if dtype == "fp16" else 0.0
     assert ((got - want).abs() <= 17 * 2.0 ** -24 + u * want + tiny).all()
+
+
+@pytest.mark.parametrize("V,dtype", [(2000, "fp32"), (2000, "bf16"), (40000, "bf16")])
+def test_log_probabilities_have_no_common_error(L, V, dtype):  # noqa: F811
+    """A sequence's reward adds up hundreds of log-probabilities, so an error of one sign counts. Each is rounded to fp32
+    below 32 in size: half a step of 2^-20 at the most, 5.5e-7 in the standard deviation, so the mean of n has
+    4.3e-9 (n = 16384) to 1.2e-8 (2048); six of those over the 5e-9 that the exponential's mean error is known to."""
+    n = 16384 if V < 10000 else 2048
+    z, y, _, _, _, _ = make(1, n, V, dtype, seed=1, mask=None)
+    got = L.logprob_rows(z, y).double()
+    want = torch.cat([torch.log_softmax(b.double(), -1).gather(-1, t[:, None])[:, 0] for b, t in zip(z[0].split(256), y[0].split(256))])
+    assert abs((got[0] - want).mean().item()) <= 6 * 2.0 ** -20 / 12 ** 0.5 / n ** 0.5 + 5e-9

@@ -101,8 +101,13 @@ __device__ __forceinline__ void update(const StepConst& k, float decay, float g,
   p = p * decay - k.step_size * __fdividef(m, root * k.root + k.eps);
 }
 
+// 1 - b^t from the fp64 logarithm of b: of b rounded to fp32 the difference would lose 1.3e-5 of itself at
+// b = 0.999, 1.4e-3 at 0.99999. (log 0 = -inf gives 1.)
+__device__ __forceinline__ float one_less_power(double log_b, int t) { return -expm1f((float)(log_b * (double)t)); }
+
 __device__ __forceinline__ StepConst step_const(const MultiHyper& h) {
-  const float t = (float)(*h.step + 1), lr = *h.lr;
+  const int t = *h.step + 1;
+  const float lr = *h.lr;
   StepConst k;
   k.b1 = h.b1;
   k.c1 = h.c1;
@@ -110,10 +115,10 @@ __device__ __forceinline__ StepConst step_const(const MultiHyper& h) {
   k.c2 = h.c2;
   k.eps = h.eps;
   k.lr = lr;
-  k.step_size = lr / (1.f - powf(h.b1, t));
-  k.root = 1.f / sqrtf(1.f - powf(h.b2, t));
+  k.step_size = lr / one_less_power(h.log_b1, t);
+  k.root = 1.f / sqrtf(one_less_power(h.log_b2, t));
   k.grad_scale = h.grad_scale * (h.grad_scale_dev ? *h.grad_scale_dev : 1.f);
-  k.seed = (uint32_t)(*h.step + 1) * 0xB7E15163u + h.seed * 0x3C6EF373u;
+  k.seed = (uint32_t)t * 0xB7E15163u + h.seed * 0x3C6EF373u;
   return k;
 }
 

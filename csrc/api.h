@@ -98,6 +98,7 @@ struct MultiState {
 };
 struct MultiHyper {
   float b1, c1, b2, c2, eps, grad_scale;  // c1 = 1 - b1, c2 = 1 - b2
+  double log_b1, log_b2;                  // natural logarithms
   const float* lr;
   const float* grad_scale_dev;  // multiplies grad_scale, or nullptr
   int* step;                    // steps taken before this one; counted by it

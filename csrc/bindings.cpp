@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "api.h"
 
@@ -395,7 +396,8 @@ struct MultiPlan {
       return 0;
     }
     llmt::MultiHyper h{(float)b1, (float)(1.0 - b1), (float)b2, (float)(1.0 - b2), (float)eps, (float)grad_scale,
-                       lr.data_ptr<float>(), static_cast<const float*>(opt_ptr(grad_scale_dev, "grad_scale")),
+                       std::log(b1), std::log(b2), lr.data_ptr<float>(),
+                       static_cast<const float*>(opt_ptr(grad_scale_dev, "grad_scale")),
                        step.data_ptr<int>(), reinterpret_cast<unsigned*>(ticket.data_ptr<int>()), (uint32_t)seed, zero_grad};
     llmt::MultiState s{m.data_ptr(), v.data_ptr(), static_cast<uint8_t*>(const_cast<void*>(opt_ptr(ms, "scale"))),
                        static_cast<uint8_t*>(const_cast<void*>(opt_ptr(vs, "scale"))), n};

@@ -91,14 +91,22 @@ struct StepConst {
   uint32_t seed;
 };
 
-// The quotient by the approximate square root and reciprocal (2^-22 of the update); the moments as written.
+// The moments as written. With 32-bit states the square root and the quotient are correctly rounded, as in adamw.cu.
+// With 8-bit states, themselves rounded to 2^-4, they are the approximate ones (2^-22 of the update; 374M values
+// 1069 us, 1097 correctly rounded), of the kind that keeps subnormal second moments: flushed to zero, those would
+// throw their weights out by lr / eps.
+template <int BITS>
 __device__ __forceinline__ void update(const StepConst& k, float decay, float g, float& p, float& m, float& v) {
   g = __fmul_rn(g, k.grad_scale);
   m = __fadd_rn(__fmul_rn(m, k.b1), __fmul_rn(g, k.c1));
   v = __fadd_rn(__fmul_rn(v, k.b2), __fmul_rn(__fmul_rn(g, k.c2), g));
-  float root;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v));
-  p = p * decay - k.step_size * __fdividef(m, root * k.root + k.eps);
+  if constexpr (BITS == 32) {
+    p = p * decay - k.step_size * (m / (sqrtf(v) * k.root + k.eps));
+  } else {
+    float root;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v));
+    p = p * decay - k.step_size * __fdividef(m, root * k.root + k.eps);
+  }
 }
 
 // 1 - b^t from the fp64 logarithm of b: of b rounded to fp32 the difference would lose 1.3e-5 of itself at
@@ -195,7 +203,7 @@ __device__ __forceinline__ void whole_block(const MultiTensor& t, const MultiHyp
   float top_m = 0.f, top_v = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    update(k, decay, g[j], p[j], m[j], v[j]);
+    update<BITS>(k, decay, g[j], p[j], m[j], v[j]);
     top_m = fmaxf(top_m, fabsf(m[j]));  // (a NaN does not set the scale)
     top_v = fmaxf(top_v, v[j]);
   }
@@ -289,7 +297,7 @@ __device__ __noinline__ void any_block(MultiTensor t, MultiHyper h, MultiState s
       m[j] = static_cast<const float*>(s.m)[si];
       v[j] = static_cast<const float*>(s.v)[si];
     }
-    update(k, decay, g, p, m[j], v[j]);
+    update<BITS>(k, decay, g, p, m[j], v[j]);
     t.p[at + i] = p;
     if (t.p16) static_cast<bf16*>(t.p16)[at + i] = __float2bfloat16_rn(p);
     if (h.zero_grad) {

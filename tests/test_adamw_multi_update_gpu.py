@@ -28,3 +28,15 @@ def test_bias_corrections(betas, bits):
             v = betas[1] * v + (1 - betas[1]) * g.double() ** 2
             want = -lr / (1 - betas[0] ** t) * m / ((v / (1 - betas[1] ** t)).sqrt() + eps)
             assert ((p[0].double() - want).abs() <= 2.0 ** -20 * want.abs()).all(), ((p[0].double() / want - 1).abs().max().item(), t)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_second_moments_below_the_normal_range(bits):
+    """Gradients of 1e-20: v = 5e-42 is 3568 units of 2^-149, held to half a unit, its root to 7.1e-5 of itself. With eps far
+    below the root the update is lr."""
+    from llmt.optim.multi import MultiAdamW
+    for n in (300, 256):  # a ragged block beside a whole one
+        p = [torch.zeros(n, device="cuda")]
+        opt = MultiAdamW(p, lr=0.5, eps=1e-30, weight_decay=0.0, state_bits=bits)
+        opt.step([torch.full((n,), 1e-20, device="cuda")])
+        assert ((p[0] + 0.5).abs() <= 0.5 * 1e-4).all(), p[0][:3]

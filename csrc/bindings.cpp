@@ -474,6 +474,7 @@ struct MultiPlan {
       }
       t.push_back({static_cast<float*>(p[i].data_ptr()), g.data_ptr(), p16.empty() ? nullptr : p16[i].data_ptr(), numel[i],
                    (int32_t)first_block[i], 0, (float)wd[i], false});
+      CHECK(t.back().p && t.back().g && (p16.empty() || t.back().p16), "adamw: tensor ", i, " has no memory (its parameter, gradient or bf16 copy was freed)");
       index.push_back((uint32_t)i);
       places[i] = (uintptr_t)t.back().p;
       if (!p16.empty()) places[p.size() + i] = (uintptr_t)t.back().p16;

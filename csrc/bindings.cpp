@@ -71,6 +71,65 @@ const void* opt_ptr(const c10::optional<at::Tensor>& t, const char* name = "oper
   return t->data_ptr();
 }
 
+// Whether two tensors share a byte, at any strides (not negative): rows (values at unit stride along the last
+// dimension, else single ones) at the distances that the other dimensions give. Searches the rows' distances, largest stride first, where what the smaller
+// strides add can still reach the other row: a few steps where strides nest, as those of heads in packed rows do.
+struct RowOverlap {
+  struct Dim {
+    int64_t stride, lo, hi;  // distance per step in bytes, steps
+  };
+  std::vector<Dim> dims;
+  std::vector<int64_t> rest_lo, rest_hi;  // what the dimensions from one on add to a distance
+  int64_t row_a = 0, row_b = 0;
+  int left = 1 << 16;  // steps; layouts that need more count as overlapping
+
+  static bool in_rows(const at::Tensor& t) { return t.dim() > 0 && t.stride(-1) == 1; }
+  static int64_t row(const at::Tensor& t) { return t.element_size() * (in_rows(t) ? t.size(-1) : 1); }
+  void add(const at::Tensor& t, int64_t sign) {
+    for (int64_t i = 0; i < t.dim() - (in_rows(t) ? 1 : 0); ++i) {
+      const int64_t s = t.stride(i) * t.element_size(), n = t.size(i) - 1;
+      if (s == 0 || n == 0) continue;
+      auto d = std::find_if(dims.begin(), dims.end(), [&](const Dim& x) { return x.stride == s; });
+      if (d == dims.end()) d = dims.insert(d, {s, 0, 0});
+      (sign > 0 ? d->hi : d->lo) += sign * n;
+    }
+  }
+  bool from(size_t k, int64_t at) {  // at: bytes from b's row to a's so far
+    if (at + rest_hi[k] <= -row_a || at + rest_lo[k] >= row_b) return false;
+    if (k == dims.size()) return true;
+    for (int64_t i = dims[k].lo; i <= dims[k].hi; ++i) {
+      const int64_t x = at + i * dims[k].stride;
+      if (x + rest_hi[k + 1] <= -row_a) {  // to the first step that reaches
+        i += std::max<int64_t>(0, (-row_a - x - rest_hi[k + 1]) / dims[k].stride - 1);
+        continue;
+      }
+      if (x + rest_lo[k + 1] >= row_b) break;
+      if (--left < 0 || from(k + 1, x)) return true;
+    }
+    return false;
+  }
+  bool operator()(const at::Tensor& a, const at::Tensor& b) {
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    row_a = row(a);
+    row_b = row(b);
+    add(a, 1);
+    add(b, -1);
+    std::sort(dims.begin(), dims.end(), [](const Dim& x, const Dim& y) { return x.stride > y.stride; });
+    rest_lo.assign(dims.size() + 1, 0);
+    rest_hi.assign(dims.size() + 1, 0);
+    for (size_t k = dims.size(); k-- > 0;) {
+      rest_lo[k] = rest_lo[k + 1] + dims[k].lo * dims[k].stride;
+      rest_hi[k] = rest_hi[k + 1] + dims[k].hi * dims[k].stride;
+    }
+    return from(0, (const char*)a.data_ptr() - (const char*)b.data_ptr());
+  }
+};
+
+void apart(const c10::optional<at::Tensor>& y, const c10::optional<at::Tensor>& x, const char* op, const char* y_name, const char* x_name) {
+  if (y.has_value() && y->defined() && x.has_value() && x->defined())
+    CHECK(!RowOverlap()(*y, *x), op, y_name, " overlaps ", x_name);
+}
+
 // ---------------------------------------------------------------- norms
 std::vector<at::Tensor> add_rmsnorm_fwd(c10::optional<at::Tensor> a, at::Tensor r, at::Tensor w, double eps,
                                         bool write_s) {
@@ -194,58 +253,6 @@ llmt::RopeHeads rope_heads(const at::Tensor& x, const at::Tensor& y) {
           y.stride(0), y.stride(1), y.stride(2),    extent(x),   extent(y)};
 }
 
-// Whether two tensors share a byte: rows of size(-1) values with unit stride along them, at any strides (not
-// negative) of the dimensions before. Searches the rows' distances, largest stride first, where what the smaller
-// strides add can still reach the other row: a few steps where strides nest, as those of heads in packed rows do.
-struct RowOverlap {
-  struct Dim {
-    int64_t stride, lo, hi;  // distance per step in bytes, steps
-  };
-  std::vector<Dim> dims;
-  std::vector<int64_t> rest_lo, rest_hi;  // what the dimensions from one on add to a distance
-  int64_t row_a = 0, row_b = 0;
-  int left = 1 << 16;  // steps; layouts that need more count as overlapping
-
-  void add(const at::Tensor& t, int64_t sign) {
-    for (int64_t i = 0; i + 1 < t.dim(); ++i) {
-      const int64_t s = t.stride(i) * t.element_size(), n = t.size(i) - 1;
-      if (s == 0 || n == 0) continue;
-      auto d = std::find_if(dims.begin(), dims.end(), [&](const Dim& x) { return x.stride == s; });
-      if (d == dims.end()) d = dims.insert(d, {s, 0, 0});
-      (sign > 0 ? d->hi : d->lo) += sign * n;
-    }
-  }
-  bool from(size_t k, int64_t at) {  // at: bytes from b's row to a's so far
-    if (at + rest_hi[k] <= -row_a || at + rest_lo[k] >= row_b) return false;
-    if (k == dims.size()) return true;
-    for (int64_t i = dims[k].lo; i <= dims[k].hi; ++i) {
-      const int64_t x = at + i * dims[k].stride;
-      if (x + rest_hi[k + 1] <= -row_a) {  // to the first step that reaches
-        i += std::max<int64_t>(0, (-row_a - x - rest_hi[k + 1]) / dims[k].stride - 1);
-        continue;
-      }
-      if (x + rest_lo[k + 1] >= row_b) break;
-      if (--left < 0 || from(k + 1, x)) return true;
-    }
-    return false;
-  }
-  bool operator()(const at::Tensor& a, const at::Tensor& b) {
-    if (a.numel() == 0 || b.numel() == 0) return false;
-    row_a = a.size(-1) * a.element_size();
-    row_b = b.size(-1) * b.element_size();
-    add(a, 1);
-    add(b, -1);
-    std::sort(dims.begin(), dims.end(), [](const Dim& x, const Dim& y) { return x.stride > y.stride; });
-    rest_lo.assign(dims.size() + 1, 0);
-    rest_hi.assign(dims.size() + 1, 0);
-    for (size_t k = dims.size(); k-- > 0;) {
-      rest_lo[k] = rest_lo[k + 1] + dims[k].lo * dims[k].stride;
-      rest_hi[k] = rest_hi[k + 1] + dims[k].hi * dims[k].stride;
-    }
-    return from(0, (const char*)a.data_ptr() - (const char*)b.data_ptr());
-  }
-};
-
 // Rotates q and (when given) k, (B, T, heads, hd) with unit stride along hd, into q_out / k_out:
 // new contiguous tensors, or given ones, which may be q and k themselves.
 std::vector<at::Tensor> rotary(at::Tensor q, c10::optional<at::Tensor> k, c10::optional<at::Tensor> positions, at::Tensor table,
@@ -302,17 +309,13 @@ std::vector<at::Tensor> rotary(at::Tensor q, c10::optional<at::Tensor> k, c10::o
   CHECK(!(q_out.has_value() && k_out.has_value() && q_out->numel() > 0 && q_out->data_ptr() == k_out->data_ptr()),
         "rotary: q_out and k_out are the same values");
   const c10::optional<at::Tensor> given_q = q, given_table = table;
-  auto apart = [&](const c10::optional<at::Tensor>& y, const c10::optional<at::Tensor>& x, const char* y_name, const char* x_name) {
-    if (!(y.has_value() && y->defined() && x.has_value() && x->defined()) || y->dim() < 1 || x->dim() < 1) return;
-    CHECK(!RowOverlap()(*y, *x), "rotary: ", y_name, " overlaps ", x_name);
-  };
-  apart(q_out, k, "q_out", "k");
-  apart(k_out, given_q, "k_out", "q");
-  apart(q_out, k_out, "q_out", "k_out");
+  apart(q_out, k, "rotary: ", "q_out", "k");
+  apart(k_out, given_q, "rotary: ", "k_out", "q");
+  apart(q_out, k_out, "rotary: ", "q_out", "k_out");
   for (auto* y : {&q_out, &k_out}) {
     const char* name = y == &q_out ? "q_out" : "k_out";
-    apart(*y, positions, name, "positions");
-    apart(*y, given_table, name, "the plan's table");
+    apart(*y, positions, "rotary: ", name, "positions");
+    apart(*y, given_table, "rotary: ", name, "the plan's table");
   }
   llmt::RopeArgs a{};
   a.B = (int)B;
@@ -735,6 +738,9 @@ std::vector<at::Tensor> policy_rows(at::Tensor logits, at::Tensor targets, c10::
   llmt::RowOut o{};
   at::Tensor d, coef, stats;
   if (grad && out.has_value()) d = gradient_rows(logits, out, o);
+  const c10::optional<at::Tensor> ids = targets, advantages = adv;
+  for (const auto& x : {std::make_pair(&ids, "targets"), {&mask, "mask"}, {&old, "old_logp"}, {&advantages, "advantages"}, {&ref, "ref_logp"}})
+    apart(out, *x.first, "", "out", x.second);
   all_on_device({{logits, "logits"}, {targets, "targets"}, {mask, "mask"}, {old, "old_logp"}, {adv, "advantages"},
                  {ref, "ref_logp"}, {out, "out"}});
   if (grad && !d.defined()) d = gradient_rows(logits, out, o);
@@ -807,6 +813,8 @@ std::vector<at::Tensor> preference_rows(at::Tensor logits, at::Tensor targets, c
   llmt::RowOut o{};
   at::Tensor d, coef, stats;
   if (grad && out.has_value()) d = gradient_rows(logits, out, o);
+  const c10::optional<at::Tensor> ids = targets;
+  for (const auto& x : {std::make_pair(&ids, "targets"), {&mask, "mask"}, {&ref, "ref_logp"}}) apart(out, *x.first, "", "out", x.second);
   all_on_device({{logits, "logits"}, {targets, "targets"}, {mask, "mask"}, {ref, "ref_logp"}, {out, "out"}});
   if (grad && !d.defined()) d = gradient_rows(logits, out, o);
   const int64_t n = (int64_t)a.B * a.T;

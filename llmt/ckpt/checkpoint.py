@@ -50,12 +50,6 @@ def _flat_opt_state(opt, flat):
         m = _full_flat(opt.exp_avg, flat.numel, world)
         v = _full_flat(opt.exp_avg_sq, flat.numel, world)
         master = _full_flat(flat.master[opt.lo:opt.hi], flat.numel, world)
-    elif hasattr(opt, "param_states"):  # MultiAdamW: its own blocks, perhaps in 8 bits
-        m = torch.zeros(flat.numel, dtype=torch.float32, device=flat.master.device)
-        v, master = torch.zeros_like(m), flat.master
-        for (a, b), o in zip(opt.param_states(), flat.offsets):
-            m[o:o + a.numel()] = a.reshape(-1)
-            v[o:o + a.numel()] = b.reshape(-1)
     else:
         m, v, master = opt.exp_avg, opt.exp_avg_sq, flat.master
     return m, v, step, master
@@ -66,11 +60,17 @@ def state_dicts(model, opt=None, flat=None):
     master = None
     st = {}
     if opt is not None and flat is not None:
-        m, v, step, master = _flat_opt_state(opt, flat)
-        for i, (p, o) in enumerate(zip(flat.params, flat.offsets)):
-            n = p.numel()
-            st[i] = {"step": torch.tensor(float(step)), "exp_avg": m[o:o + n].view(p.shape).cpu().clone(),
-                     "exp_avg_sq": v[o:o + n].view(p.shape).cpu().clone()}
+        if hasattr(opt, "tensor_state"):  # MultiAdamW: its own blocks, perhaps in 8 bits, decoded one tensor at a time
+            step, master = int(opt.step_t.item()), flat.master
+            for i in range(len(flat.params)):
+                a, b = (x.cpu() for x in opt.tensor_state(i))
+                st[i] = {"step": torch.tensor(float(step)), "exp_avg": a, "exp_avg_sq": b}
+        else:
+            m, v, step, master = _flat_opt_state(opt, flat)
+            for i, (p, o) in enumerate(zip(flat.params, flat.offsets)):
+                n = p.numel()
+                st[i] = {"step": torch.tensor(float(step)), "exp_avg": m[o:o + n].view(p.shape).cpu().clone(),
+                         "exp_avg_sq": v[o:o + n].view(p.shape).cpu().clone()}
     sd = {}
     for k, t in model.state_dict().items():
         sd[k] = t.detach().cpu().clone()

@@ -83,27 +83,43 @@ class MultiAdamW:
                                                 dtype == torch.float32))
 
     # ------------------------------------------------------------------ checkpoints
+    def tensor_state(self, i):
+        """(exp_avg, exp_avg_sq) of tensor i, fp32 in its shape: decoded from its own blocks, with 32-bit
+        states views of them."""
+        p, b = self.params[i], self.plan.first_block[i]
+        k = -(-p.numel() // BLOCK)
+        at, n = slice(b * BLOCK, (b + k) * BLOCK), p.numel()
+        m, v = self.exp_avg[at], self.exp_avg_sq[at]
+        if self.state_bits == 8:
+            m, v = N.ext().adamw_state_values(m, self.exp_avg_scale[b:b + k], v, self.exp_avg_sq_scale[b:b + k], True)
+        return m[:n].view(p.shape), v[:n].view(p.shape)
+
+    def load_tensor_state(self, i, exp_avg, exp_avg_sq):
+        """Inverse of tensor_state, from any device. Values that came from 8-bit states are taken over exactly, others
+        are rounded to the nearest."""
+        p, b = self.params[i], self.plan.first_block[i]
+        k = -(-p.numel() // BLOCK)
+        at, n = slice(b * BLOCK, (b + k) * BLOCK), p.numel()
+        m, v = self.exp_avg[at], self.exp_avg_sq[at]
+        if self.state_bits == 32:
+            m[:n].copy_(exp_avg.reshape(-1))
+            v[:n].copy_(exp_avg_sq.reshape(-1))
+            return
+        full = torch.zeros((2, k * BLOCK), dtype=torch.float32, device=m.device)
+        full[0, :n].copy_(exp_avg.reshape(-1))
+        full[1, :n].copy_(exp_avg_sq.reshape(-1))
+        N.ext().adamw_encode_states(full[0], full[1], m, self.exp_avg_scale[b:b + k], v, self.exp_avg_sq_scale[b:b + k])
+
     def param_states(self):
-        """[(exp_avg, exp_avg_sq)] per tensor, fp32 in its shape (torch.optim.AdamW's layout)."""
-        m, v = self.state_values(torch.float32)
-        out = []
-        for p, b in zip(self.params, self.plan.first_block):
-            at = slice(b * BLOCK, b * BLOCK + p.numel())
-            out.append((m[at].view(p.shape).clone(), v[at].view(p.shape).clone()))
-        return out
+        """[(exp_avg, exp_avg_sq)] per tensor, fp32 in its shape (torch.optim.AdamW's layout), all at once: 8 bytes a value.
+        A checkpoint of a model that fits only with 8-bit states takes tensor_state one by one."""
+        return [tuple(x.clone() if self.state_bits == 32 else x for x in self.tensor_state(i)) for i in range(len(self.params))]
 
     def load_param_states(self, states):
-        """Inverse of param_states; an entry None leaves that tensor's states. Values that came from
-        8-bit states are taken over exactly, others are rounded to the nearest."""
-        m, v = self.state_values(torch.float32)
-        for p, b, s in zip(self.params, self.plan.first_block, states):
-            if s is None:
-                continue
-            at = slice(b * BLOCK, b * BLOCK + p.numel())
-            m[at].copy_(s[0].reshape(-1))
-            v[at].copy_(s[1].reshape(-1))
-        if self.state_bits == 8:
-            N.ext().adamw_encode_states(m, v, self.exp_avg, self.exp_avg_scale, self.exp_avg_sq, self.exp_avg_sq_scale)
+        """Inverse of param_states, tensor by tensor; an entry None leaves that tensor's states."""
+        for i, s in zip(range(len(self.params)), states):
+            if s is not None:
+                self.load_tensor_state(i, *s)
 
     def state_dict(self, flat=None):
         """torch.optim.AdamW-style state, the moments in fp32."""

@@ -458,7 +458,7 @@ cudaError_t launch(const MultiTensor* t, int count, const MultiHyper& h, const M
 
 template <typename G, int BITS>
 cudaError_t launches(const MultiTensor* t, int count, const MultiHyper& h, const MultiState& s, cudaStream_t st) {
-  constexpr int kSmall = 64, kLarge = 640;  // 3.1 KB and 30.7 KB of kernel arguments
+  constexpr int kSmall = 64, kLarge = kTensorsPerLaunch;  // 3.1 KB and 30.7 KB of kernel arguments
   for (int i = 0; i < count; i += kLarge) {
     const int k = std::min(kLarge, count - i);
     const bool last = i + k == count;

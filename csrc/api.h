@@ -106,6 +106,7 @@ struct MultiHyper {
   uint32_t seed;
   bool zero_grad;
 };
+constexpr int kTensorsPerLaunch = 640;  // 30.7 KB of kernel arguments; more tensors take several launches
 cudaError_t adamw_multi(const MultiTensor* t, int count, bool grad_bf16, int bits, const MultiHyper& h, const MultiState& s,
                         cudaStream_t st);
 // n: a multiple of 8, outputs bf16 or fp32 (f32).
@@ -138,6 +139,8 @@ struct TokenBatch {
   Strided<int64_t> tgt;
   Strided<uint8_t> mask;
 };
+// Batches of at most this many tokens, averaged over tokens, are counted by each row's CTA; others by a kernel.
+constexpr int kTokensCountedInRows = 512;
 enum LossReduction : int { LOSS_TOKEN = 0, LOSS_SEQUENCE = 1, LOSS_SUM = 2 };
 enum PreferenceKind : int { PREF_SIGMOID = 0, PREF_HINGE = 1, PREF_IPO = 2 };
 struct PolicyArgs {

@@ -444,7 +444,7 @@ struct MultiPlan {
     for (size_t i = 1; i < spans.size(); ++i) CHECK(spans[i].first >= spans[i - 1].second, "adamw: two tensors share memory");
   }
 
-  // grads: one per tensor, None leaves that tensor and its states as they are.
+  // grads: one per tensor, None leaves that tensor and its states as they are. Returns the kernels launched.
   int64_t step(const pybind11::list& grads, int64_t bits, at::Tensor m, at::Tensor v, c10::optional<at::Tensor> ms,
                c10::optional<at::Tensor> vs, at::Tensor lr, at::Tensor step, at::Tensor ticket, double b1, double b2, double eps,
                double grad_scale, c10::optional<at::Tensor> grad_scale_dev, int64_t seed, bool zero_grad) {
@@ -520,7 +520,7 @@ struct MultiPlan {
     llmt::MultiState s{m.data_ptr(), v.data_ptr(), static_cast<uint8_t*>(const_cast<void*>(opt_ptr(ms, "scale"))),
                        static_cast<uint8_t*>(const_cast<void*>(opt_ptr(vs, "scale"))), n};
     ok(llmt::adamw_multi(t.data(), (int)t.size(), bf16, (int)bits, h, s, stream()), "adamw_multi");
-    return 1;
+    return ((int64_t)t.size() + llmt::kTensorsPerLaunch - 1) / llmt::kTensorsPerLaunch;
   }
 };
 
@@ -1260,6 +1260,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "q_out"_a = py::none(), "k_out"_a = py::none());
   m.def("loss_error_code", &llmt::loss_error_code, "reset"_a = false);
   m.def("logprob_rows", &logprob_rows, "logits"_a, "targets"_a, "mask"_a = py::none());
+  m.attr("tokens_counted_in_rows") = (int)llmt::kTokensCountedInRows;
   m.def("policy_rows", &policy_rows, "logits"_a, "targets"_a, "old"_a, "adv"_a, "ref"_a, "mask"_a, "clip_lo"_a,
         "clip_hi"_a, "kl"_a, "reduction"_a, "grad"_a, "out"_a = py::none(), "keep"_a = false);
   m.def("policy_tokens", &policy_tokens, "logp"_a, "targets"_a, "V"_a, "old"_a, "adv"_a, "ref"_a, "mask"_a, "clip_lo"_a,

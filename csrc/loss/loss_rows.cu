@@ -196,11 +196,10 @@ __global__ void __launch_bounds__(256) count_tokens_kernel(TokenBatch a, int* co
   }
 }
 
-// Batches of at most this many tokens, averaged over tokens, are counted by each row's CTA while its row is on
-// the way, in place of a kernel before it (the call for 80 rows 16.2 -> 14.4 us of host time).
-constexpr int kCountHere = 512;
+// Few tokens, averaged over tokens, are counted by each row's CTA while its row is on the way, in place of a
+// kernel before it (the call for 80 rows 16.2 -> 14.4 us of host time).
 __host__ __device__ inline bool counted_here(const TokenBatch& a, int reduction) {
-  return reduction == LOSS_SUM || (reduction == LOSS_TOKEN && (int64_t)a.B * a.T <= kCountHere);
+  return reduction == LOSS_SUM || (reduction == LOSS_TOKEN && (int64_t)a.B * a.T <= kTokensCountedInRows);
 }
 __device__ __forceinline__ float token_weight_here(const TokenBatch& a, int reduction) {  // by one warp
   if (reduction == LOSS_SUM) return 1.f;

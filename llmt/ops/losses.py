@@ -76,8 +76,11 @@ def logprob_rows(logits, targets, mask=None):
 
 def _policy_rows(logits, targets, old_logp, advantages, ref_logp, mask, clip, kl_coef, reduction, grad, out=None, keep=False):
     lo, hi = _clip(clip)
-    return N.ext().policy_rows(logits, targets, old_logp, advantages, ref_logp, mask, lo, hi, float(kl_coef),
-                               _choice(REDUCTIONS, reduction, "reduction"), bool(grad), out, keep)
+    C = N.ext()
+    if reduction == "sequence" or (reduction == "token" and targets.numel() > C.tokens_counted_in_rows):
+        N.LAUNCHES.count += 1  # the kernel that counts the tokens
+    return C.policy_rows(logits, targets, old_logp, advantages, ref_logp, mask, lo, hi, float(kl_coef),
+                         _choice(REDUCTIONS, reduction, "reduction"), bool(grad), out, keep)
 
 
 def policy_loss_rows(logits, targets, old_logp, advantages, ref_logp=None, mask=None, clip=(0.2, 0.2), kl_coef=0.0,
@@ -108,6 +111,7 @@ def preference_loss_rows(logits, targets, ref_logp=None, mask=None, beta=0.1, ki
         hinge:   max(0, 1 - beta D)
         ipo:     (D - 1 / (2 beta))^2
     averaged over pairs. Returns PreferenceRows(loss, logp, rewards = beta * gains (2 P), dlogits)."""
+    N.LAUNCHES.count += 1 if grad else 0  # the gradient's rows
     loss, logp, rewards, d, _, _ = N.ext().preference_rows(
         logits, targets, ref_logp, mask, float(beta), float(label_smoothing), _choice(KINDS, kind, "kind"), bool(average),
         bool(grad), out)

@@ -21,7 +21,9 @@ EPI_BF16, EPI_F32, EPI_SWIGLU, EPI_SWIGLU_BWD, EPI_ROPE, EPI_CE_FWD, EPI_CE_BWD 
 _KERNELS_PER_CALL = {"flash_attn_bwd": 3, "gemm_error_code": 0, "attn_error_code": 0, "loss_error_code": 0, "dp_error_code": 0,
                      "set_reserved_sms": 0, "reserved_sms": 0,
                      "ipc_alloc": 0, "ipc_open": 0, "ipc_close": 0, "ipc_free": 0, "tensor_from_ptr": 0,
-                     "sm_count": 0, "MultiPlan": 0, "bounds_error": 0, "bounds_checking": 0, "fp8_quant": 2, "fp8_amax_slots": 0, "mx_sf_bytes": 0, "gemm_plan": 0}
+                     "sm_count": 0, "MultiPlan": 0, "bounds_error": 0, "bounds_checking": 0, "fp8_quant": 2, "fp8_amax_slots": 0, "mx_sf_bytes": 0, "gemm_plan": 0,
+                     # the row kernels and their sum (or the pairs' losses); what else a call launches is counted by llmt.ops.losses
+                     "policy_rows": 2, "policy_tokens": 2, "preference_rows": 2}
 
 
 class LaunchCounter:
@@ -49,7 +51,8 @@ class _Counted:
 
     def __getattr__(self, name):
         fn = getattr(self._mod, name)
-        if not callable(fn):
+        if not callable(fn):  # a constant of the build
+            self.__dict__[name] = fn
             return fn
         k = _KERNELS_PER_CALL.get(name, 1)
 

@@ -703,7 +703,8 @@ __global__ void __launch_bounds__(kPairThreads) preference_kernel(TokenBatch a, 
   float loss, slope;  // of the pair, slope in D
   if (q.kind == PREF_SIGMOID) {
     const float s = q.smoothing, soft = log1pf(expf(-fabsf(x)));
-    loss = (1.f - s) * (soft + fmaxf(-x, 0.f)) + s * (soft + fmaxf(x, 0.f));
+    loss = (1.f - s) * (soft + fmaxf(-x, 0.f));
+    if (s > 0.f) loss += s * (soft + fmaxf(x, 0.f));  // (0 times the infinity of an impossible rejected token is 0)
     slope = q.beta * (s / (1.f + expf(-x)) - (1.f - s) / (1.f + expf(x)));
   } else if (q.kind == PREF_HINGE) {
     loss = x != x ? x : fmaxf(0.f, 1.f - x);

@@ -247,8 +247,9 @@ __device__ __forceinline__ void policy_token(const PolicyArgs& q, PolicyToken k,
   // an advantage of zero takes no part, a ratio past fp32 included (inf * 0 would be NaN)
   const float free = A == 0.f ? 0.f : r * A;
   const float held = A == 0.f ? 0.f : fminf(fmaxf(r, 1.f - q.clip_lo), 1.f + q.clip_hi) * A;
-  // a NaN ratio or advantage stays one in the loss and in the slope: fminf, fmaxf and comparisons drop it
-  const bool bad = r != r || A != A;
+  // a NaN ratio or advantage, or an infinite advantage under a ratio of zero, is one in the loss and in the slope:
+  // fminf, fmaxf and comparisons drop it
+  const bool bad = r != r || free != free;
   float l = bad ? NAN : -(free <= held ? free : held);
   float c = bad ? NAN : free <= held ? -free : 0.f;
   if (q.ref.p) {

@@ -35,3 +35,13 @@ def test_an_impossible_token_of_a_rejected_sequence(L, form, kind, smoothing):  
         assert abs(r.loss.item() - one.loss.item() / 2) <= 2.0 ** -23 * one.loss.item()
         assert (grad[[1, 3]] == 0).all()
     assert grad.isfinite().all() and (grad[[0, 2]] != 0).any()
+
+
+def test_an_infinite_advantage_shows_in_the_gradient(L):  # noqa: F811
+    """Also under a ratio that is zero in fp32, e^-200."""
+    z, y, _, old, _, adv = make(1, 4, 300, "fp32", mask=None)
+    adv[0, 1], adv[0, 2] = float("inf"), float("inf")
+    old[0, 1] = 200.0
+    r = L.policy_loss_rows(z, y, old, adv, reduction="sum")
+    assert not r.loss.isfinite() and not r.dlogits[0, 1].isfinite().any() and not r.dlogits[0, 2].isfinite().any()
+    assert r.dlogits[0, [0, 3]].isfinite().all()

@@ -30,6 +30,8 @@ class MultiAdamW:
         b1, b2 = betas
         if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
             raise ValueError(f"betas must be in [0, 1), not {betas}")
+        if not eps >= 0.0:
+            raise ValueError(f"eps must be at least 0, not {eps}")
         params = [p.detach() for p in params]
         wd = [float(w) for w in weight_decay] if isinstance(weight_decay, (list, tuple)) else [float(weight_decay)] * len(params)
         self.plan = N.ext().MultiPlan(params, [s.detach() for s in shadows] if shadows is not None else [], wd)

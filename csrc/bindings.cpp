@@ -308,14 +308,16 @@ std::vector<at::Tensor> rotary(at::Tensor q, c10::optional<at::Tensor> k, c10::o
     }
   CHECK(!(q_out.has_value() && k_out.has_value() && q_out->numel() > 0 && q_out->data_ptr() == k_out->data_ptr()),
         "rotary: q_out and k_out are the same values");
-  const c10::optional<at::Tensor> given_q = q, given_table = table;
-  apart(q_out, k, "rotary: ", "q_out", "k");
-  apart(k_out, given_q, "rotary: ", "k_out", "q");
-  apart(q_out, k_out, "rotary: ", "q_out", "k_out");
-  for (auto* y : {&q_out, &k_out}) {
-    const char* name = y == &q_out ? "q_out" : "k_out";
-    apart(*y, positions, "rotary: ", name, "positions");
-    apart(*y, given_table, "rotary: ", name, "the plan's table");
+  if (q_out.has_value() || k_out.has_value()) {
+    const c10::optional<at::Tensor> given_q = q, given_table = table;
+    apart(q_out, k, "rotary: ", "q_out", "k");
+    apart(k_out, given_q, "rotary: ", "k_out", "q");
+    apart(q_out, k_out, "rotary: ", "q_out", "k_out");
+    for (auto* y : {&q_out, &k_out}) {
+      const char* name = y == &q_out ? "q_out" : "k_out";
+      apart(*y, positions, "rotary: ", name, "positions");
+      apart(*y, given_table, "rotary: ", name, "the plan's table");
+    }
   }
   llmt::RopeArgs a{};
   a.B = (int)B;
@@ -738,9 +740,11 @@ std::vector<at::Tensor> policy_rows(at::Tensor logits, at::Tensor targets, c10::
   llmt::RowOut o{};
   at::Tensor d, coef, stats;
   if (grad && out.has_value()) d = gradient_rows(logits, out, o);
-  const c10::optional<at::Tensor> ids = targets, advantages = adv;
-  for (const auto& x : {std::make_pair(&ids, "targets"), {&mask, "mask"}, {&old, "old_logp"}, {&advantages, "advantages"}, {&ref, "ref_logp"}})
-    apart(out, *x.first, "", "out", x.second);
+  if (out.has_value()) {
+    const c10::optional<at::Tensor> ids = targets, advantages = adv;
+    for (const auto& x : {std::make_pair(&ids, "targets"), {&mask, "mask"}, {&old, "old_logp"}, {&advantages, "advantages"}, {&ref, "ref_logp"}})
+      apart(out, *x.first, "", "out", x.second);
+  }
   all_on_device({{logits, "logits"}, {targets, "targets"}, {mask, "mask"}, {old, "old_logp"}, {adv, "advantages"},
                  {ref, "ref_logp"}, {out, "out"}});
   if (grad && !d.defined()) d = gradient_rows(logits, out, o);
@@ -813,8 +817,10 @@ std::vector<at::Tensor> preference_rows(at::Tensor logits, at::Tensor targets, c
   llmt::RowOut o{};
   at::Tensor d, coef, stats;
   if (grad && out.has_value()) d = gradient_rows(logits, out, o);
-  const c10::optional<at::Tensor> ids = targets;
-  for (const auto& x : {std::make_pair(&ids, "targets"), {&mask, "mask"}, {&ref, "ref_logp"}}) apart(out, *x.first, "", "out", x.second);
+  if (out.has_value()) {
+    const c10::optional<at::Tensor> ids = targets;
+    for (const auto& x : {std::make_pair(&ids, "targets"), {&mask, "mask"}, {&ref, "ref_logp"}}) apart(out, *x.first, "", "out", x.second);
+  }
   all_on_device({{logits, "logits"}, {targets, "targets"}, {mask, "mask"}, {ref, "ref_logp"}, {out, "out"}});
   if (grad && !d.defined()) d = gradient_rows(logits, out, o);
   const int64_t n = (int64_t)a.B * a.T;

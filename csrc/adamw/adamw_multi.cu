@@ -342,7 +342,7 @@ __device__ __forceinline__ int find_tensor(const Batch<CAP>& batch, int64_t w, i
 }
 
 // Bound by memory: with 32-bit states 28 to 30 bytes a value, 103% of the measured copy rate for 0.94G values
-// (3.90 ms); with 8-bit states 16 to 18 bytes, 97% for 374M values (1.06 ms), at 72% of the issue slots.
+// (3.89 ms); with 8-bit states 16 to 18 bytes, 97% for 374M values (1.07 ms), at 76% of the issue slots.
 // A CTA takes a run of `rounds` blocks a warp, consecutive warps consecutive blocks, and ends: the memory
 // serves a few hundred short runs, handed out in order, at its copy rate, but a persistent grid at 88%
 // (4.57 ms), whether it sweeps through all tensors together or each CTA steps through runs of its own.

@@ -19,7 +19,7 @@
 // through two 32 KB tiles of shared memory by bulk copies, summing one while the next arrives, and
 // goes back from the last tile to the first for the gradient: the last two are still there, the others are
 // read again from L2 or memory. Three CTAs of 256 threads a SM work on different rows. (2 x 32 KB and 3 CTAs
-// 337 us for 4 x 1024 x 128256 bf16; 3 x 32 KB and 2 CTAs 342, 4 x 16 KB 363, 2 x 24 KB and 4 CTAs 355; a row held
+// 338 us for 4 x 1024 x 128256 bf16; 3 x 32 KB and 2 CTAs 342, 4 x 16 KB 363, 2 x 24 KB and 4 CTAs 355; a row held
 // by a cluster of 64 KB slices, read once but waited for as a whole, 410; gradients stored without the streaming
 // hint 357.) Where there are few rows a cluster of up to 8 CTAs shares one, and exchanges the maximum and
 // sum of each warp through distributed shared memory. Sums, maxima and slopes are fp32, the sums over
@@ -450,8 +450,9 @@ struct Tiles {
 };
 
 // One cluster per row: its maximum, sum and log-probability; with POLICY the loss and slope of its
-// token, with GRAD also the row of the gradient. The row lies in shared memory from its one read to its
-// gradient; the CTAs on a SM work on different rows, so that one's copy runs under another's arithmetic.
+// token, with GRAD also the row of the gradient, which goes back over the row's tiles: a slice of up to two is
+// still in shared memory, of longer ones the tiles before the last two are read again. The CTAs on a SM work on
+// different rows, so that one's copy runs under another's arithmetic.
 template <typename T, int THREADS, bool POLICY, bool GRAD>
 __global__ void __launch_bounds__(THREADS, 768 / THREADS) token_rows_kernel(TokenBatch a, PolicyArgs q, RowOut o, int ctas) {
   constexpr int kWarps = THREADS / 32;

@@ -6,8 +6,9 @@ vocabulary; the logits of the others are not read and get a zero gradient. Witho
 counts a policy loss is 0 and a sequence's gain is 0.
 
   logprob_rows           log-probabilities of the targets
-  policy_loss_rows       loss, log-probabilities and the gradient of the logits in one call: the
-  preference_loss_rows   logits are read once (twice for the pairs, whose slopes need both sums)
+  policy_loss_rows       loss, log-probabilities and the gradient of the logits in one call: logits of
+  preference_loss_rows   rows up to 64 KB are read once (twice for the pairs, whose slopes need both
+                         sums); of longer rows what lies before the last 64 KB a second time, in part from L2
   policy_loss            the same behind autograd; the gradient goes to the logits
   preference_loss
   policy_loss_tokens     the losses on log-probabilities that a fused head gives

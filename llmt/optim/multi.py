@@ -4,8 +4,10 @@ The update is FusedAdamW's (torch.optim.AdamW's), for tensors that need not lie 
 each with its own weight decay. With state_bits=8 the two moments take 2 bytes and 2/256 per value
 in place of 8: blocks of 256 values under a power-of-two scale, the first moment in e4m3, the second
 in eight unsigned bits (csrc/adamw/adamw_multi.cu), rounded up or down with probabilities that keep their
-mean. The random bits are a hash of the value's place, the step count and the seed: the same run
-gives the same bits. A NaN gradient makes its value and its first moment NaN, as in 32 bits.
+mean. An update is computed from the moments before that rounding, with the approximate square root
+and quotient (2^-22 of it; with 32-bit states both are correctly rounded). The random bits are a hash
+of the value's place, the step count and the seed: the same run gives the same bits. A NaN gradient
+makes its value and its first moment NaN, as in 32 bits.
 
 lr and the step count live on the device, so `step()` can be captured in a CUDA graph and replayed.
 """

@@ -12,7 +12,7 @@ def launches(fn):
     fn()
     torch.cuda.synchronize()
     before = LAUNCHES.count
-    with profile(activities=[ProfilerActivity.CUDA]) as prof:
+    with profile(activities=[ProfilerActivity.CUDA], acc_events=True) as prof:
         fn()
         torch.cuda.synchronize()
     counted = LAUNCHES.count - before

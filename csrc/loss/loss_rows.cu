@@ -323,7 +323,7 @@ __device__ __forceinline__ void fill_tile(const RowView<T>& in, const Slice<T, T
   const int wb = max(b, in.whole_lo), we = min(e, in.whole_hi);
   if (threadIdx.x == 0) {
     const uint32_t bytes = we > wb ? (uint32_t)(we - wb) * 16u : 0u;
-    const bool inside = LLMT_IN(in.at + wb * RowView<T>::N - in.off, in.at + max(we, wb) * RowView<T>::N - in.off, in.n, 601);
+    const bool inside = bytes == 0 || LLMT_IN(in.at + wb * RowView<T>::N - in.off, in.at + we * RowView<T>::N - in.off, in.n, 601);
     sm100::bar_arrive_expect_tx(bar, inside ? bytes : 0u);
     if (bytes && inside) {
       const T* src = in.p + (wb * RowView<T>::N - in.off);
@@ -346,8 +346,8 @@ __device__ __forceinline__ void store_pieces(const RowView<T>& out, const RowVie
   }
   const int we = min(e, out.whole_hi);
   uint4* const base = out.piece(0);
-  const bool inside = LLMT_IN(out.at + (int64_t)max(b, out.whole_lo) * Piece<T>::N - out.off,
-                              out.at + (int64_t)max(max(b, out.whole_lo), we) * Piece<T>::N - out.off, out.n, 603);
+  const int wb = max(b, out.whole_lo);
+  const bool inside = we <= wb || LLMT_IN(out.at + (int64_t)wb * Piece<T>::N - out.off, out.at + (int64_t)we * Piece<T>::N - out.off, out.n, 603);
   if (inside) {
 #pragma unroll 4
     for (int i = b + (int)threadIdx.x; i < we; i += THREADS) {
